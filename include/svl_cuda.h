@@ -363,6 +363,112 @@ SVL_API svl_status svl_rvq_encode_device(svl_rvq* rvq, int32_t batch, int32_t fr
                                          const float* d_latent, uint32_t* d_codes,
                                          void* cuda_stream);
 
+/* ---- The 8-bit step's operators ----
+ *
+ * e4m3 rows with one f32 scale per row and block of 128 columns: value (r, c) stands for
+ * e4m3(d_q[r * q_stride + c]) * d_scales[(c / 128) * scale_stride + r]. They have no
+ * counterpart in the reference, whose weights are f32, bf16 or Q8_0.
+ *
+ * `device` is the GPU that holds the tensors (it need not be the current one, which a call leaves
+ * as it was), `cuda_stream` a stream of it (NULL = its default stream). Calls only enqueue work,
+ * allocate nothing and may be captured into graphs; zero rows are no work. Strides count
+ * elements. Outputs must not overlap inputs except where a call says so. */
+
+/* h = x + residual; y = norm(h); y as e4m3 rows.
+ *   d_x, d_residual (NULL = none), d_sum (h; NULL = not kept): [rows][k] of `dtype`
+ *   (SVL_DT_F32 or SVL_DT_BF16). h is rounded to dtype, and the norm reads the rounded value.
+ *   d_sum may be d_x or d_residual itself (same pointer and stride).
+ *   norm_kind: SVL_NORM_RMS (h / sqrt(mean(h^2) + eps) * weight), SVL_NORM_LAYER
+ *   ((h - mean) / sqrt(var + eps) * weight + bias) or -1 (y = h); d_weight and d_bias are f32
+ *   [k], NULL = ones and zeros.
+ *   Per block: a = max(max |y|, 2^-100), scale = a / 448, q = e4m3(y * (448 / a)), rounded to
+ *   nearest even. A block that holds a NaN or an infinity stands for NaN.
+ * q_stride is a multiple of 16 bytes (svl_f8_linear_device reads the rows with TMA), k at most
+ * 32,768 (SVL_ERR_UNSUPPORTED above). Columns [k, q_stride) are left as they were. */
+SVL_API svl_status svl_add_norm_f8_device(int32_t device, int64_t rows, int32_t k, int32_t dtype,
+                                          const void* d_x, int64_t x_stride,
+                                          const void* d_residual, int64_t residual_stride,
+                                          int32_t norm_kind, const float* d_weight,
+                                          const float* d_bias, float eps, void* d_sum,
+                                          int64_t sum_stride, uint8_t* d_q, int64_t q_stride,
+                                          float* d_scales, int64_t scale_stride,
+                                          void* cuda_stream);
+
+/* A weight matrix [n][k] as e4m3 with one f32 scale per block of 128 rows x 128 columns, laid
+ * out for svl_f8_linear_device. Immutable; may be shared by threads and streams. */
+typedef struct svl_f8_linear svl_f8_linear;
+/* From host f32 tensors "weight" [n][k] and (optional) "bias" [n]: scale = max(max |w|, 2^-100)
+ * / 448 of the block, q = e4m3(w * (448 / max)), rounded to nearest even. */
+SVL_API svl_status svl_f8_linear_create(int32_t n, int32_t k, const svl_tensor_view* tensors,
+                                        int32_t n_tensors, int32_t device, svl_f8_linear** out);
+/* From e4m3 weights on the device: d_weight [n] rows, weight_stride bytes apart, d_scales
+ * [ceil(n / 128)][ceil(k / 128)], d_bias [n] or NULL. Copied after the work on cuda_stream, which
+ * the call waits for. */
+SVL_API svl_status svl_f8_linear_create_device(int32_t n, int32_t k, const uint8_t* d_weight,
+                                               int64_t weight_stride, const float* d_scales,
+                                               const float* d_bias, int32_t device,
+                                               void* cuda_stream, svl_f8_linear** out);
+SVL_API void svl_f8_linear_destroy(svl_f8_linear* linear);
+/* out[r][j] = sum over blocks b of scale(r, b) * weight scale(j / 128, b) * (sum of the block's
+ * products) + bias[j], summed in f32 and rounded once to out_dtype (SVL_DT_F32 or SVL_DT_BF16).
+ * The rows are svl_add_norm_f8_device's: d_q 16-byte aligned, q_stride a multiple of 16 and at
+ * least k. A row's result does not depend on timing; it may depend on the number of rows of the
+ * call, which chooses how the sums over k are split. */
+SVL_API svl_status svl_f8_linear_device(svl_f8_linear* linear, int64_t rows, const uint8_t* d_q,
+                                        int64_t q_stride, const float* d_scales,
+                                        int64_t scale_stride, int32_t out_dtype, void* d_out,
+                                        int64_t out_stride, void* cuda_stream);
+/* Waits for the device, then SVL_ERR_TIMEOUT if a bounded device-side wait of a product of this
+ * matrix ran out (its outputs are then undefined), SVL_OK otherwise; the flag is cleared. */
+SVL_API svl_status svl_f8_linear_error(svl_f8_linear* linear);
+
+/* Rules between logits and token, device memory; a null pointer leaves a rule out.
+ *   Penalties: d_history [rows][history_stride] holds each row's ring of history_cap (at most
+ *   65,535) past tokens; d_lengths [rows] counts the tokens ever recorded: the first
+ *   min(length, history_cap) entries count, in any order. Ids outside the vocabulary (pads) and
+ *   ids below first_penalised do not count. A token that occurs c > 0 times: l = l > 0 ?
+ *   l / repetition : l * repetition, then l = l - (frequency * c + presence). d_repetition (1),
+ *   d_frequency (0) and d_presence (0) are [rows] f32.
+ *   Biases: l = l + d_dense_bias[v] ([vocab], every row's), then l = l + d_bias_values[r][i] for
+ *   each i < bias_cap (at most 65,535) with d_bias_ids[r][i] == v, in order; ids outside the
+ *   vocabulary are pads. bias_stride counts both arrays' rows.
+ *   Grammar: bit v % 32 of word v / 32 of row d_mask_rows[r] (r itself when null) of d_masks
+ *   [n_masks][mask_stride] says whether token v may follow; -infinity where not. A mask row
+ *   outside [0, n_masks) means no grammar.
+ *   append: the picked token is recorded at d_history[r][length % history_cap] and the length
+ *   counted up (not for tokens below first_penalised, nor where there is none). */
+typedef struct svl_logits_rules {
+  int32_t* d_history;
+  int64_t history_stride;
+  int32_t* d_lengths;
+  int32_t history_cap;
+  int32_t first_penalised;
+  const float* d_repetition;
+  const float* d_frequency;
+  const float* d_presence;
+  const float* d_dense_bias;
+  const int32_t* d_bias_ids;
+  const float* d_bias_values;
+  int64_t bias_stride;
+  int32_t bias_cap;
+  int32_t n_masks;
+  const uint32_t* d_masks;
+  int64_t mask_stride;
+  const int32_t* d_mask_rows;
+  int32_t append;
+  int32_t _pad;
+} svl_logits_rules;
+
+/* The rules (NULL = none) on logits [rows][logits_stride] of `dtype` (SVL_DT_F32 or
+ * SVL_DT_BF16), computed in f32: d_out [rows][out_stride] of the same dtype (NULL = not kept;
+ * may be d_logits itself, with its stride) and d_tokens [rows] (NULL = not wanted): the lowest
+ * index of the largest value, -1 where no value is above -infinity (NaN never is). */
+SVL_API svl_status svl_logits_rules_device(int32_t device, int64_t rows, int32_t vocab,
+                                           int32_t dtype, const void* d_logits,
+                                           int64_t logits_stride, const svl_logits_rules* rules,
+                                           void* d_out, int64_t out_stride, int32_t* d_tokens,
+                                           void* cuda_stream);
+
 /* Message of the last failure on this thread ("" when none). */
 SVL_API const char* svl_last_error(void);
 SVL_API const char* svl_version(void);

@@ -22,6 +22,7 @@ STATUS = {0: "OK", 1: "CONFIG", 2: "INVALID_INPUT", 3: "CUDA", 4: "OOM", 5: "TIM
 # Every symbol of include/svl_cuda.h with its (restype, argtypes).
 _P = ctypes.c_void_p
 _I = ctypes.c_int32
+_L = ctypes.c_int64
 _U32P = ctypes.POINTER(ctypes.c_uint32)
 _F32P = ctypes.POINTER(ctypes.c_float)
 SIGNATURES = {
@@ -67,6 +68,14 @@ SIGNATURES = {
     "svl_rvq_create": (_I, [_I, _I, _P, _I, _I, ctypes.POINTER(_P)]),
     "svl_rvq_destroy": (None, [_P]),
     "svl_rvq_encode_device": (_I, [_P, _I, _I, _P, _P, _P]),
+    "svl_add_norm_f8_device": (_I, [_I, _L, _I, _I, _P, _L, _P, _L, _I, _P, _P, ctypes.c_float, _P, _L, _P,
+                                    _L, _P, _L, _P]),
+    "svl_f8_linear_create": (_I, [_I, _I, ctypes.POINTER(CTensorView), _I, _I, ctypes.POINTER(_P)]),
+    "svl_f8_linear_create_device": (_I, [_I, _I, _P, _L, _P, _P, _I, _P, ctypes.POINTER(_P)]),
+    "svl_f8_linear_destroy": (None, [_P]),
+    "svl_f8_linear_device": (_I, [_P, _L, _P, _L, _P, _L, _I, _P, _L, _P]),
+    "svl_f8_linear_error": (_I, [_P]),
+    "svl_logits_rules_device": (_I, [_I, _L, _I, _I, _P, _L, _P, _P, _L, _P, _P]),
     "svl_last_error": (ctypes.c_char_p, []),
     "svl_version": (ctypes.c_char_p, []),
 }
