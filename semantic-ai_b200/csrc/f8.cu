@@ -20,9 +20,6 @@ __device__ __forceinline__ void store_stream(__nv_bfloat16* p, float v) { *p = _
 __device__ __forceinline__ uint8_t to_e4m3(float v) {
   return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
 }
-__device__ __forceinline__ float from_e4m3(uint8_t v) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(v, __NV_E4M3)));
-}
 // Maximum that keeps a NaN.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -142,48 +139,6 @@ __global__ void __launch_bounds__(256) f8_quantise_kernel(const float* src, int 
   if (threadIdx.x == 0) scales[(int64_t)tile * kblocks + kb] = top / kF8Max;
 }
 
-// 16 rows x 64 matrix rows per CTA of 256 threads, one 128-column block at a time: its products
-// are summed apart, then scaled into the running sum.
-constexpr int kTR = 16, kTN = 64;
-__global__ void __launch_bounds__(256) f8_gemm_simple_kernel(const F8GemmParams p) {
-  __shared__ float xs[kTR][kF8Block + 1], ws[kTN][kF8Block + 1];
-  const int kblocks = p.m.kblocks();
-  const int n0 = blockIdx.x * kTN, t = threadIdx.x, tn = t & 63, tr = t >> 6;
-  for (int64_t r0 = (int64_t)blockIdx.y * kTR; r0 < p.rows; r0 += (int64_t)gridDim.y * kTR) {
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int b = 0; b < kblocks; b++) {
-      __syncthreads();
-      for (int i = t; i < kTR * kF8Block; i += 256) {
-        const int64_t r = r0 + i / kF8Block;
-        const int c = b * kF8Block + i % kF8Block;
-        xs[i / kF8Block][i % kF8Block] = r < p.rows && c < p.m.k ? from_e4m3(p.q[r * p.q_stride + c]) : 0.f;
-      }
-      for (int i = t; i < kTN * kF8Block; i += 256) {
-        const int n = n0 + i / kF8Block, c = b * kF8Block + i % kF8Block;
-        ws[i / kF8Block][i % kF8Block] = n < p.m.n && c < p.m.k ? from_e4m3(p.m.w[packed_at(n, c, kblocks)]) : 0.f;
-      }
-      __syncthreads();
-      const float sw = p.m.scales[(int64_t)(n0 / kF8Block) * kblocks + b];
-      for (int j = 0; j < 4; j++) {
-        const int64_t r = r0 + tr + 4 * j;
-        float s = 0.f;
-        for (int c = 0; c < kF8Block; c++) s = fmaf(xs[tr + 4 * j][c], ws[tn][c], s);
-        if (r < p.rows) acc[j] = fmaf(s, p.scales[(int64_t)b * p.scale_stride + r] * sw, acc[j]);
-      }
-    }
-    const int n = n0 + tn;
-    for (int j = 0; j < 4; j++) {
-      const int64_t r = r0 + tr + 4 * j;
-      if (r >= p.rows || n >= p.m.n) continue;
-      const float y = acc[j] + (p.m.bias ? p.m.bias[n] : 0.f);
-      if (p.out_bf16)
-        static_cast<__nv_bfloat16*>(p.out)[r * p.out_stride + n] = __float2bfloat16_rn(y);
-      else
-        static_cast<float*>(p.out)[r * p.out_stride + n] = y;
-    }
-  }
-}
-
 }  // namespace
 
 void launch_norm_f8(const NormF8Params& p, cudaStream_t s) {
@@ -206,12 +161,6 @@ void launch_f8_quantise(const float* src, int n, int k, int interleave_half, uin
   const dim3 grid((k + kF8Block - 1) / kF8Block, (n + kF8Block - 1) / kF8Block);
   f8_quantise_kernel<<<grid, 256, 0, s>>>(src, n, k, interleave_half, dst, scales);
   check_cuda(cudaGetLastError(), "quantise launch");
-}
-
-void launch_f8_gemm(const F8GemmParams& p, cudaStream_t s) {
-  const dim3 grid((p.m.n + kTN - 1) / kTN, (unsigned)std::min<int64_t>((p.rows + kTR - 1) / kTR, 32768));
-  f8_gemm_simple_kernel<<<grid, 256, 0, s>>>(p);
-  check_cuda(cudaGetLastError(), "product launch");
 }
 
 }  // namespace svl

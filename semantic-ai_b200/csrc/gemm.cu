@@ -25,6 +25,7 @@
 #include "common.cuh"
 #include "kernels.cuh"
 #include "sm100.cuh"
+#include "tcgen05.cuh"
 
 namespace svl {
 namespace {
@@ -51,60 +52,6 @@ struct Cfg {
   static_assert((size_t)kBM * BN * 4 <= (size_t)kStages * kStage, "epilogue must fit the ring");
 };
 
-// ---- tcgen05 / TMA wrappers ---------------------------------------------------------------
-
-// Shared-memory matrix descriptor: K-major, 128-byte swizzle, 8-row groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (1ull << 16) | (64ull << 32) | (1ull << 46) |
-         (2ull << 61);
-}
-// Instruction descriptor of kind::f16: f32 accumulator, A and B both bf16 (fmt 1) or both
-// f16 (fmt 0), both K-major.
-__host__ __device__ constexpr uint32_t idesc_f16kind(int m, int n, uint32_t fmt) {
-  return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(n >> 3) << 17) |
-         ((uint32_t)(m >> 4) << 24);
-}
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* tm, int c0, int c1,
-                                            uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_addr(dst)),
-      "l"(reinterpret_cast<uint64_t>(tm)), "r"(c0), "r"(c1), "r"(smem_addr(bar))
-      : "memory");
-}
-__device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc,
-                                          uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   smem_addr(bar))
-               : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-// 16 consecutive f32 columns of this thread's TMEM lane.
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
-  uint32_t r[16];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-      "%11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
-}
 // Order-preserving map of a float onto an unsigned key (larger float, larger key).
 __device__ __forceinline__ uint32_t order_key(float v) {
   const uint32_t u = __float_as_uint(v);
@@ -600,23 +547,6 @@ __global__ void __launch_bounds__(kPrepThreads) prep_kernel(const float* x, int6
 
 // ---- host side ----------------------------------------------------------------------------
 
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                 const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiled encoder() {
-  static EncodeTiled fn = [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q{};
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      return (EncodeTiled) nullptr;
-    return reinterpret_cast<EncodeTiled>(f);
-  }();
-  return fn;
-}
-
 template <int BN, int EPI>
 void launch_be(const GemmOperand& w, const GemmOperand& x, const GemmArgs& ga, int tiles,
                int stream_tiles, cudaStream_t s) {
@@ -671,7 +601,7 @@ void set_attrs_bn() {
 bool make_gemm_operand(GemmOperand& op, const void* base, int rows, int k, int64_t row_bytes,
                        int box_rows, int f16) {
   static_assert(sizeof(op.map) >= sizeof(CUtensorMap), "tensor map storage");
-  EncodeTiled enc = encoder();
+  const EncodeTiled enc = tma_encoder();
   if (!enc || !base || rows <= 0 || k <= 0 || row_bytes % 16 || box_rows > 256 || box_rows < 8 ||
       reinterpret_cast<uintptr_t>(base) % 16)
     return false;
@@ -694,7 +624,7 @@ bool make_gemm_operand(GemmOperand& op, const void* base, int rows, int k, int64
 
 bool make_ring_map(unsigned char* map128, const void* base, int64_t rows, int head_dim, int layers,
                    int64_t layer_stride, int box_rows) {
-  EncodeTiled enc = encoder();
+  const EncodeTiled enc = tma_encoder();
   if (!enc || !base || rows <= 0 || head_dim % 64 || layers <= 0 || (layer_stride * 2) % 16 ||
       box_rows > 256 || box_rows < 1 || reinterpret_cast<uintptr_t>(base) % 16)
     return false;
