@@ -1,4 +1,5 @@
-"""Builds libsvl_b200.so (the sm_100a kernels and the C ABI) in-tree with nvcc.
+"""Builds libsvl_b200.so (the sm_100a kernels and the C ABI) in-tree with nvcc, and the operators'
+binding to torch tensors (svl/_torch_ops.so) with the host compiler.
 
 Run `python semantic-ai_b200/build.py` or call build(). Objects go to semantic-ai_b200/_build/,
 the library to semantic-ai_b200/libsvl_b200.so. Only sources newer than their object are
@@ -16,6 +17,8 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 OUT = PKG / "_build"
 LIB = PKG / "libsvl_b200.so"
+TORCH_SRC = CSRC / "torch_ops.cpp"
+TORCH_OPS = PKG / "svl" / "_torch_ops.so"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 # -fmad=false: no implicit a*b+c contraction, so element-wise arithmetic rounds like the
@@ -51,11 +54,33 @@ def _compile(src: Path, extra: list[str]) -> Path:
     return obj
 
 
+def _build_torch_ops() -> None:
+    newest = max(TORCH_SRC.stat().st_mtime, (PKG.parent / "include" / "svl_cuda.h").stat().st_mtime)
+    if TORCH_OPS.exists() and TORCH_OPS.stat().st_mtime >= newest:
+        return
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    # nvcc's own host compiler, as for the library: another one's C++ library may not be torch's.
+    cmd = [NVCC, "-std=c++17", "-O2", "-shared", "-cudart", "none", "-Xcompiler", "-fPIC,-fvisibility=hidden,-w",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-isystem", str(root / "include"), "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
+           "-isystem", sysconfig.get_paths()["include"], str(TORCH_SRC), "-o", str(TORCH_OPS),
+           "-L", str(root / "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"building {TORCH_OPS.name} failed:\n{r.stdout}\n{r.stderr}")
+
+
 def build(verbose: bool = False, extra: list[str] | None = None) -> Path:
     OUT.mkdir(exist_ok=True)
     extra = extra or []
     with cf.ThreadPoolExecutor(max_workers=os.cpu_count() or 4) as ex:
+        ops = ex.submit(_build_torch_ops)
         objs = list(ex.map(lambda s: _compile(s, extra), _sources()))
+        ops.result()
     if LIB.exists() and LIB.stat().st_mtime >= max(o.stat().st_mtime for o in objs):
         return LIB
     cmd = [NVCC, "-shared", "-gencode", "arch=compute_100a,code=sm_100a",

@@ -4,12 +4,7 @@ from __future__ import annotations
 
 import ctypes
 
-import torch
-
-from . import _lib
-from .f8 import _DTYPES, _row_stride, _rows, _stream, _vector
-
-_INTS = (torch.int32,)
+from ._ops import ops, raw_stream
 
 
 class CLogitsRules(ctypes.Structure):
@@ -37,58 +32,5 @@ def logits_rules(logits, history=None, lengths=None, repetition=None, frequency=
     dense_bias float32 [vocab]; bias_ids int32 and bias_values float32 [rows, entries] (ids
     outside the vocabulary are pads). masks int32 [n, words of 32 tokens], a set bit allows its
     token; mask_rows int32 [rows] chooses a row's mask (-1: none; without it, row r takes mask r)."""
-    _rows("logits", logits)
-    rows, vocab = logits.shape
-    device = logits.device
-    r = CLogitsRules()
-    if history is not None or lengths is not None:
-        if history is None or lengths is None:
-            raise ValueError("history and lengths go together")
-        _rows("history", history, (rows, history.shape[1]), _INTS)
-        _same(device, history=history)
-    if history is not None and (history.shape[1] or append):
-        r.d_history, r.history_stride, r.history_cap = history.data_ptr(), _row_stride(history), history.shape[1]
-        r.d_lengths = _ints("lengths", lengths, rows, device)
-    r.d_repetition = _vector("repetition", repetition, rows, device)
-    r.d_frequency = _vector("frequency", frequency, rows, device)
-    r.d_presence = _vector("presence", presence, rows, device)
-    r.d_dense_bias = _vector("dense_bias", dense_bias, vocab, device)
-    if bias_ids is not None or bias_values is not None:
-        if bias_ids is None or bias_values is None:
-            raise ValueError("bias_ids and bias_values go together")
-        _rows("bias_ids", bias_ids, (rows, bias_ids.shape[1]), _INTS)
-        _rows("bias_values", bias_values, bias_ids.shape, (torch.float32,))
-        _same(device, bias_ids=bias_ids, bias_values=bias_values)
-        if rows > 1 and bias_ids.stride(0) != bias_values.stride(0):
-            raise ValueError("bias_ids and bias_values must have the same row stride")
-        r.d_bias_ids, r.d_bias_values = bias_ids.data_ptr(), bias_values.data_ptr()
-        r.bias_stride, r.bias_cap = _row_stride(bias_ids), bias_ids.shape[1]
-    if masks is not None:
-        _rows("masks", masks, (masks.shape[0], max(masks.shape[1], (vocab + 31) // 32)), _INTS)
-        _same(device, masks=masks)
-        r.d_masks, r.mask_stride, r.n_masks = masks.data_ptr(), _row_stride(masks), masks.shape[0]
-    if mask_rows is not None:
-        r.d_mask_rows = _ints("mask_rows", mask_rows, rows, device)
-    r.first_penalised, r.append = first_penalised, int(append)
-    if out is None:
-        out = torch.empty((rows, vocab), dtype=logits.dtype, device=device)
-    else:
-        _rows("out", out, logits.shape, (logits.dtype,))
-        _same(device, out=out)
-    tokens = torch.empty((rows,), dtype=torch.int32, device=device)
-    _lib.check(_lib.lib().svl_logits_rules_device(
-        device.index, rows, vocab, _DTYPES[logits.dtype], logits.data_ptr(), _row_stride(logits), ctypes.byref(r),
-        out.data_ptr(), _row_stride(out), tokens.data_ptr(), _stream(stream, device)))
-    return out, tokens
-
-
-def _same(device, **tensors):
-    for name, t in tensors.items():
-        if t.device != device:
-            raise ValueError(f"{name} is on {t.device}, the logits on {device}")
-
-
-def _ints(name: str, t, n: int, device):
-    if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{name} must be {n} contiguous int32 values on {device}: got {tuple(t.shape)}, {t.dtype}, {t.device}")
-    return t.data_ptr()
+    return ops.logits_rules(logits, history, lengths, repetition, frequency, presence, dense_bias, bias_ids, bias_values,
+                            masks, mask_rows, first_penalised, append, out, raw_stream(stream))
