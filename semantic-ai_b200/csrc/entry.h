@@ -2,6 +2,7 @@
 // C-ABI call from what it throws, and the caller's current device kept.
 #pragma once
 
+#include <atomic>
 #include <new>
 
 #include "engine.h"
@@ -54,5 +55,17 @@ class OnDevice {
   int before_ = 0;
   bool moved_ = false;
 };
+
+// Raises a kernel's dynamic shared-memory limit, once per device (the attribute is the device's).
+template <auto kernel>
+void allow_smem(size_t bytes) {
+  static std::atomic<uint64_t> done{0};
+  int device = 0;
+  check_cuda(cudaGetDevice(&device), "cudaGetDevice");
+  const uint64_t bit = 1ull << (device & 63);
+  if (device < 64 && (done.load(std::memory_order_acquire) & bit)) return;
+  check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "shared memory");
+  if (device < 64) done.fetch_or(bit, std::memory_order_release);
+}
 
 }  // namespace svl

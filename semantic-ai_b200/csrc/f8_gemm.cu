@@ -18,7 +18,7 @@
 #include <cuda_bf16.h>
 
 #include "common.cuh"
-#include "engine.h"
+#include "entry.h"
 #include "f8.cuh"
 #include "tcgen05.cuh"
 
@@ -537,10 +537,10 @@ bool make_rows_map(CUtensorMap* map, const uint8_t* base, int64_t rows, int k, i
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <class K>
-void launch(K kernel, dim3 grid, int threads, size_t smem, int split, const CUtensorMap& map, const F8Args& a,
+template <auto kernel>
+void launch(dim3 grid, int threads, size_t smem, int split, const CUtensorMap& map, const F8Args& a,
             cudaStream_t s) {
-  check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "product");
+  allow_smem<kernel>(smem);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -572,7 +572,7 @@ void launch_thin(F8Args a, cudaStream_t s) {
   a.ntiles = a.p.m.tiles();
   a.rtiles = (int)((a.p.rows + BN - 1) / BN);
   a.split = choose_split((int64_t)a.ntiles * a.rtiles, a.kblocks, 2 * 148, 1);
-  launch(f8_thin_kernel<BN>, dim3(a.ntiles * a.split, a.rtiles), Thin<BN>::kThreads, Thin<BN>::kSmem, a.split, map, a, s);
+  launch<f8_thin_kernel<BN>>(dim3(a.ntiles * a.split, a.rtiles), Thin<BN>::kThreads, Thin<BN>::kSmem, a.split, map, a, s);
 }
 
 template <int TN>
@@ -586,7 +586,7 @@ void launch_wide(F8Args a, cudaStream_t s) {
   if (tiles > INT32_MAX) throw Error(SVL_ERR_UNSUPPORTED, "too many output tiles");
   a.split = choose_split(tiles, a.kblocks, 148, 2);
   const int grid = a.split > 1 ? (int)tiles * a.split : (int)std::min<int64_t>(tiles, 148);
-  launch(f8_wide_kernel<TN>, dim3(grid), Wide<TN>::kThreads, Wide<TN>::kSmem, a.split, map, a, s);
+  launch<f8_wide_kernel<TN>>(dim3(grid), Wide<TN>::kThreads, Wide<TN>::kSmem, a.split, map, a, s);
 }
 
 }  // namespace
