@@ -8,14 +8,10 @@
 #include "common.cuh"
 #include "entry.h"
 #include "f8.cuh"
+#include "sm100.cuh"
 
 namespace svl {
 namespace {
-
-__device__ __forceinline__ float load_stream(const float* p) { return *p; }
-__device__ __forceinline__ float load_stream(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ void store_stream(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store_stream(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
 __device__ __forceinline__ uint8_t to_e4m3(float v) {
   return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
@@ -27,74 +23,161 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-constexpr int kNormThreads = 256;
+// Eight consecutive values of a row of the stream as f32; `have` of them exist.
+template <class T>
+__device__ __forceinline__ void load8(const T* p, int have, bool wide, float (&v)[8]) {
+  if (wide && have == 8) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+      const uint4 a = *reinterpret_cast<const uint4*>(p);
+      v[0] = bf16_lo(a.x); v[1] = bf16_hi(a.x); v[2] = bf16_lo(a.y); v[3] = bf16_hi(a.y);
+      v[4] = bf16_lo(a.z); v[5] = bf16_hi(a.z); v[6] = bf16_lo(a.w); v[7] = bf16_hi(a.w);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = j < have ? (float)p[j] : 0.f;
+  }
+}
+template <class T>
+__device__ __forceinline__ void store8(T* p, int have, bool wide, const float (&v)[8]) {
+  if (wide && have == 8) {
+    if constexpr (sizeof(T) == 4) {
+      reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      __nv_bfloat162 h[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) h[j] = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+      *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(h);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      if (j < have) p[j] = sizeof(T) == 4 ? (T)v[j] : (T)__float2bfloat16_rn(v[j]);
+  }
+}
 
-__device__ float block_sum(float v, float* red) {
+// The sum of v over a row's threads (a multiple of 32, threadIdx.x of them): warp sums, then the
+// warps' sums in order. `red` belongs to the row; its barrier is 1 + threadIdx.y.
+__device__ __forceinline__ float row_sum(float v, float* red) {
   v = warp_sum(v);
-  __syncthreads();
+  const int warps = blockDim.x >> 5;
+  if (warps == 1) return v;
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float s = 0.f;
-  for (int w = 0; w < kNormThreads / 32; w++) s += red[w];
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + threadIdx.y), "r"(blockDim.x) : "memory");
+  float s = red[0];
+  for (int w = 1; w < warps; w++) s += red[w];
   return s;
 }
 
-// One CTA per row, the row in shared memory.
-template <class T>
-__global__ void __launch_bounds__(kNormThreads) norm_f8_kernel(const NormF8Params p) {
-  extern __shared__ float row[];
-  __shared__ float red[kNormThreads / 32];
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
-    const T* x = static_cast<const T*>(p.x) + r * p.x_stride;
-    const T* res = p.residual ? static_cast<const T*>(p.residual) + r * p.residual_stride : nullptr;
-    T* sum = p.sum ? static_cast<T*>(p.sum) + r * p.sum_stride : nullptr;
+// A row's threads (threadIdx.x) hold the whole row in registers, I pieces of 8 values each, so x
+// and the residual are read once: bound by HBM. 16 consecutive threads hold a block of 128
+// columns, whose maximum takes four shuffles. Short rows share a CTA (threadIdx.y).
+template <class T, int I>
+__global__ void __launch_bounds__(I == 4 ? 1024 : 512) norm_f8_kernel(const NormF8Params p) {
+  __shared__ float red_sm[2][32];
+  const int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  pdl_launch();
+  pdl_wait();
+  if (r >= p.rows) return;
+  // A CTA's rows use disjoint parts of red (blockDim.x / 32 * blockDim.y <= 32 warps).
+  float* red = red_sm[0] + threadIdx.y * (blockDim.x >> 5);
+  float* red2 = red_sm[1] + threadIdx.y * (blockDim.x >> 5);
+  const T* x = static_cast<const T*>(p.x) + r * p.x_stride;
+  const T* res = p.residual ? static_cast<const T*>(p.residual) + r * p.residual_stride : nullptr;
+  T* sum = p.sum ? static_cast<T*>(p.sum) + r * p.sum_stride : nullptr;
+  const bool xw = reinterpret_cast<uintptr_t>(x) % 16 == 0, rw = reinterpret_cast<uintptr_t>(res) % 16 == 0,
+             sw = reinterpret_cast<uintptr_t>(sum) % 16 == 0;
+  const bool ww = reinterpret_cast<uintptr_t>(p.weight) % 16 == 0, bw = reinterpret_cast<uintptr_t>(p.bias) % 16 == 0;
+  float h[I][8];
+#pragma unroll
+  for (int i = 0; i < I; i++) {
+    const int c = (threadIdx.x + i * blockDim.x) * 8;
+    load8(x + c, min(8, p.k - c), xw, h[i]);
+  }
+  if (res) {
+#pragma unroll
+    for (int i = 0; i < I; i++) {
+      const int c = (threadIdx.x + i * blockDim.x) * 8;
+      float a[8];
+      load8(res + c, min(8, p.k - c), rw, a);
+#pragma unroll
+      for (int j = 0; j < 8; j++) h[i][j] = sizeof(T) == 4 ? h[i][j] + a[j] : round_bf16(h[i][j] + a[j]);
+    }
+  }
+  if (sum) {
+#pragma unroll
+    for (int i = 0; i < I; i++) {
+      const int c = (threadIdx.x + i * blockDim.x) * 8;
+      store8(sum + c, min(8, p.k - c), sw, h[i]);
+    }
+  }
+  if (p.norm != NORM_NONE) {
     float a = 0.f;
-    for (int i = t; i < p.k; i += kNormThreads) {
-      float h = load_stream(x + i);
-      if (res) h = h + load_stream(res + i);
-      if (sizeof(T) == 2) h = round_bf16(h);
-      if (sum) store_stream(sum + i, h);
-      row[i] = h;
-      a += p.norm == NORM_LAYER ? h : h * h;
-    }
-    float mean = 0.f, rstd = 1.f;
-    if (p.norm != NORM_NONE) {
-      a = block_sum(a, red) / (float)p.k;
-      if (p.norm == NORM_LAYER) {
-        mean = a;
-        float c = 0.f;
-        for (int i = t; i < p.k; i += kNormThreads) c += (row[i] - mean) * (row[i] - mean);
-        a = block_sum(c, red) / (float)p.k;
+    if (p.norm == NORM_LAYER) {
+#pragma unroll
+      for (int i = 0; i < I; i++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) a += h[i][j];
+      const float mean = row_sum(a, red2) / (float)p.k;
+#pragma unroll
+      for (int i = 0; i < I; i++) {
+        const int c = (threadIdx.x + i * blockDim.x) * 8;
+#pragma unroll
+        for (int j = 0; j < 8; j++) h[i][j] = c + j < p.k ? h[i][j] - mean : 0.f;
       }
-      rstd = 1.0f / sqrtf(a + p.eps);
+      a = 0.f;
     }
-    __syncthreads();
-    for (int b = warp; b * kF8Block < p.k; b += kNormThreads / 32) {
-      float y[4], top = 0.f;
-      for (int j = 0; j < 4; j++) {
-        const int i = b * kF8Block + j * 32 + lane;
-        y[j] = 0.f;
-        if (i < p.k) {
-          y[j] = row[i];
-          if (p.norm != NORM_NONE) {
-            y[j] = (y[j] - mean) * rstd;
-            if (p.weight) y[j] = y[j] * p.weight[i];
-            if (p.bias && p.norm == NORM_LAYER) y[j] = y[j] + p.bias[i];
-          }
-        }
-        top = max_nan(top, fabsf(y[j]));
+#pragma unroll
+    for (int i = 0; i < I; i++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) a = fmaf(h[i][j], h[i][j], a);
+    const float rstd = 1.0f / sqrtf(row_sum(a, red) / (float)p.k + p.eps);
+#pragma unroll
+    for (int i = 0; i < I; i++) {
+      const int c = (threadIdx.x + i * blockDim.x) * 8, have = min(8, p.k - c);
+#pragma unroll
+      for (int j = 0; j < 8; j++) h[i][j] = h[i][j] * rstd;
+      float a8[8];
+      if (p.weight) {
+        load8(p.weight + c, have, ww, a8);
+#pragma unroll
+        for (int j = 0; j < 8; j++) h[i][j] = h[i][j] * a8[j];
       }
-      for (int o = 16; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-      top = max_nan(top, kF8Tiny);
-      const float inv = kF8Max / top;
-      for (int j = 0; j < 4; j++) {
-        const int i = b * kF8Block + j * 32 + lane;
-        if (i < p.k) p.q[r * p.q_stride + i] = to_e4m3(y[j] * inv);
+      if (p.bias && p.norm == NORM_LAYER) {
+        load8(p.bias + c, have, bw, a8);
+#pragma unroll
+        for (int j = 0; j < 8; j++) h[i][j] = h[i][j] + a8[j];
       }
-      if (lane == 0) p.scales[(int64_t)b * p.scale_stride + r] = top / kF8Max;
     }
-    __syncthreads();
+  }
+  uint8_t* q = p.q + r * p.q_stride;
+#pragma unroll
+  for (int i = 0; i < I; i++) {
+    const int c = (threadIdx.x + i * blockDim.x) * 8, have = p.k - c;
+    float top = kF8Tiny;
+#pragma unroll
+    for (int j = 0; j < 8; j++) top = max_nan(top, j < have ? fabsf(h[i][j]) : 0.f);
+#pragma unroll
+    for (int o = 8; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float inv = __fdiv_rn(kF8Max, top);
+    if (have >= 8) {
+      uint2 v;
+      uint16_t* e = reinterpret_cast<uint16_t*>(&v);
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        e[j] = __nv_cvt_float2_to_fp8x2(make_float2(h[i][2 * j] * inv, h[i][2 * j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+      *reinterpret_cast<uint2*>(q + c) = v;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        if (j < have) q[c + j] = to_e4m3(h[i][j] * inv);
+    }
+    if ((threadIdx.x & 15) == 0 && have > 0)
+      p.scales[(int64_t)(c / kF8Block) * p.scale_stride + r] = __fdiv_rn(top, kF8Max);
   }
 }
 
@@ -141,14 +224,27 @@ __global__ void __launch_bounds__(256) f8_quantise_kernel(const float* src, int 
 
 }  // namespace
 
+// Pieces per thread: one up to 4,096 columns (512 threads), then two and four, so that a CTA stays
+// small enough for several per SM; rows below 2,048 columns share CTAs of 256 threads.
 void launch_norm_f8(const NormF8Params& p, cudaStream_t s) {
-  const int grid = (int)std::min<int64_t>(p.rows, 148 * 64);
-  const size_t smem = (size_t)p.k * 4;
-  auto kernel = p.bf16 ? norm_f8_kernel<__nv_bfloat16> : norm_f8_kernel<float>;
-  if (smem > 48 * 1024)
-    check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "norm");
-  kernel<<<grid, kNormThreads, smem, s>>>(p);
-  check_cuda(cudaGetLastError(), "norm launch");
+  const int pieces = (p.k + 7) / 8;
+  const int per = pieces <= 512 ? 1 : pieces <= 1024 ? 2 : 4;
+  const int threads = ((pieces + per - 1) / per + 31) / 32 * 32;
+  const int share = (int)std::min<int64_t>(std::max(1, 256 / threads), p.rows);
+  const int64_t grid = (p.rows + share - 1) / share;
+  if (grid > INT32_MAX) throw Error(SVL_ERR_UNSUPPORTED, "too many rows");
+  auto kernel = p.bf16 ? (per == 1 ? norm_f8_kernel<__nv_bfloat16, 1> : per == 2 ? norm_f8_kernel<__nv_bfloat16, 2> : norm_f8_kernel<__nv_bfloat16, 4>)
+                       : (per == 1 ? norm_f8_kernel<float, 1> : per == 2 ? norm_f8_kernel<float, 2> : norm_f8_kernel<float, 4>);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(threads, share);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  check_cuda(cudaLaunchKernelEx(&cfg, kernel, p), "norm launch");
 }
 
 void launch_f8_pack(const uint8_t* src, int64_t stride, int n, int k, uint8_t* dst, cudaStream_t s) {
