@@ -41,9 +41,14 @@ struct F8Args {
   int rtiles;        // tiles along the rows
 };
 
+// The MMA issuer's and the loader's loops are single threads, a block of them has to take less than
+// the block's product (512 clocks for 128 x 256), so they keep shared-memory addresses and
+// descriptors in registers and count stages instead of dividing.
+
 // A role's bounded wait; a wait that ran out marks the CTA as failed.
-__device__ __forceinline__ bool role_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
-  if (mbar_wait(bar, parity)) return true;
+__device__ __forceinline__ bool role_wait(uint32_t bar, uint32_t parity, int* failed) {
+  for (uint32_t i = 0; i < kWaitLimit; i++)
+    if (mbar_try_wait_at(bar, parity)) return true;
   *failed = 1;
   return false;
 }
@@ -62,32 +67,33 @@ __device__ __forceinline__ void drain_mma(uint64_t* bar) {
 // ---- few rows: matrix rows are the MMA's M, up to BN rows its N ------------------------------
 
 // Bound by the weights' bytes: every CTA keeps a ring of about 100 KB of loads in flight, two
-// CTAs per SM.
+// CTAs per SM (one with 192 KB for 128 rows). A stage of the ring, its TMEM buffer and its scales
+// share one index and one phase: `full` (loaded), `done` (multiplied: the stage may be loaded
+// again, the buffer read), `read` (the epilogue is through with buffer and scales).
 template <int BN>
 struct Thin {
   static constexpr int kEpiWarps = BN <= 64 ? 4 : 8;
   static constexpr int kThreads = (kEpiWarps + 3) * 32;  // + loader, MMA issuer, scales
   static constexpr uint32_t kXBytes = BN * kF8Block;
   static constexpr uint32_t kStage = kTile + kXBytes;
-  static constexpr int kStages = (int)(106 * 1024 / kStage);
-  static constexpr int kBufs = BN <= 32 ? 4 : 2;
-  static constexpr uint32_t kCols = BN * kBufs < 32 ? 32 : BN * kBufs;
-  static constexpr int kScaleSlots = 8;
+  static constexpr int kStages = BN == 16 ? 6 : BN == 32 ? 5 : BN == 64 ? 4 : 4;
+  static constexpr uint32_t kCols = BN == 16 ? 128 : BN == 32 ? 256 : BN == 64 ? 256 : 512;
   static constexpr size_t kRing = (size_t)kStages * kStage;
-  static constexpr size_t kSmem = kRing + kScaleSlots * BN * 4 + 1024;
+  static constexpr size_t kSmem = kRing + kStages * BN * 4 + 1024;
   static constexpr int kCpt = BN / (kEpiWarps / 4);  // columns (rows of x) per epilogue thread
-  static_assert((size_t)(BN + kMaxSplit) * kF8Block * 4 <= kRing, "the exchange reuses the ring");
+  static constexpr int kLd = kCpt < 32 ? 16 : 32;    // columns per TMEM load
+  static_assert(kStages * BN <= (int)kCols, "a TMEM buffer per stage");
+  static_assert((size_t)(BN + 4 * kMaxSplit) * kF8Block * 4 <= kRing, "the exchange reuses the ring");
 };
 
 template <int BN>
-__global__ void __launch_bounds__(Thin<BN>::kThreads) f8_thin_kernel(const __grid_constant__ CUtensorMap tm_x,
-                                                                     const __grid_constant__ F8Args a) {
+__global__ void __launch_bounds__(Thin<BN>::kThreads, BN <= 64 ? 2 : 1)
+    f8_thin_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ F8Args a) {
   using C = Thin<BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* scale_ring = reinterpret_cast<float*>(smem + C::kRing);
-  __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages], tfull[C::kBufs], tempty[C::kBufs],
-      sfull[C::kScaleSlots], sempty[C::kScaleSlots], gone;
+  __shared__ __align__(8) uint64_t full[C::kStages], done[C::kStages], read[C::kStages], scaled[C::kStages], gone;
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
   const F8GemmParams& p = a.p;
@@ -102,15 +108,9 @@ __global__ void __launch_bounds__(Thin<BN>::kThreads) f8_thin_kernel(const __gri
   if (tid == 0) {
     for (int i = 0; i < C::kStages; i++) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
-    }
-    for (int i = 0; i < C::kBufs; i++) {
-      mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], C::kEpiWarps);
-    }
-    for (int i = 0; i < C::kScaleSlots; i++) {
-      mbar_init(&sfull[i], 1);
-      mbar_init(&sempty[i], C::kEpiWarps);
+      mbar_init(&done[i], 1);
+      mbar_init(&read[i], C::kEpiWarps);
+      mbar_init(&scaled[i], 1);
     }
     mbar_init(&gone, 1);
     failed = 0;
@@ -122,9 +122,9 @@ __global__ void __launch_bounds__(Thin<BN>::kThreads) f8_thin_kernel(const __gri
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  float acc[C::kCpt];
+  uint64_t acc[C::kCpt / 2];
 #pragma unroll
-  for (int i = 0; i < C::kCpt; i++) acc[i] = 0.f;
+  for (int i = 0; i < C::kCpt / 2; i++) acc[i] = 0;
 
   if (warp == C::kEpiWarps) {
     if (lane == 0) {
@@ -138,13 +138,19 @@ __global__ void __launch_bounds__(Thin<BN>::kThreads) f8_thin_kernel(const __gri
       pdl_wait();
       for (int i = 0; i < pre; i++)
         tma_load_2d(smem + (size_t)i * C::kStage + kTile, &tm_x, (b0 + i) * kF8Block, r0, &full[i]);
-      int i = pre;
+      w += (int64_t)pre * kF8TileBytes;
+      int i = pre, st = 0;
+      uint32_t parity = 0;
       for (; i < nb; i++) {
-        const int st = i % C::kStages;
-        if (!role_wait(&empty[st], ((i / C::kStages) - 1) & 1, &failed)) break;
+        if (!role_wait(smem_addr(&done[st]), parity, &failed)) break;
         mbar_expect_tx(&full[st], C::kStage);
-        bulk_g2s(smem + (size_t)st * C::kStage, w + i * kF8TileBytes, kTile, &full[st]);
+        bulk_g2s(smem + (size_t)st * C::kStage, w, kTile, &full[st]);
         tma_load_2d(smem + (size_t)st * C::kStage + kTile, &tm_x, (b0 + i) * kF8Block, r0, &full[st]);
+        w += kF8TileBytes;
+        if (++st == C::kStages) {
+          st = 0;
+          parity ^= 1;
+        }
       }
       pdl_launch();
       drain_loads(full, i, C::kStages);
@@ -152,81 +158,88 @@ __global__ void __launch_bounds__(Thin<BN>::kThreads) f8_thin_kernel(const __gri
   } else if (warp == C::kEpiWarps + 1) {
     if (lane == 0) {
       constexpr uint32_t idesc = idesc_e4m3(kF8Block, BN);
-      for (int i = 0; i < nb; i++) {
-        const int st = i % C::kStages, buf = i % C::kBufs;
-        if (i >= C::kBufs && !role_wait(&tempty[buf], ((i / C::kBufs) - 1) & 1, &failed)) break;
-        if (!role_wait(&full[st], (i / C::kStages) & 1, &failed)) break;
-        tc_fence_after();
-        const uint32_t wa = smem_addr(smem + (size_t)st * C::kStage), xa = wa + kTile;
+      const uint32_t full_at = smem_addr(full), read_at = smem_addr(read);
+      const uint64_t w_desc = sw128_desc(smem_addr(smem)), x_desc = sw128_desc(smem_addr(smem) + kTile);
+      uint32_t parity = 0;
+      bool ok = true;
+      for (int left = nb; left > 0 && ok; left -= C::kStages, parity ^= 1) {
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-          umma_f8(tmem + buf * BN, sw128_desc(wa + k * 32), sw128_desc(xa + k * 32), idesc, k != 0);
-        umma_commit(&empty[st]);
-        umma_commit(&tfull[buf]);
+        for (int st = 0; st < C::kStages; st++) {
+          if (st >= left || !ok) break;
+          ok = role_wait(read_at + 8 * st, parity ^ 1, &failed) && role_wait(full_at + 8 * st, parity, &failed);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < 4; k++)
+            umma_f8(tmem + st * BN, w_desc + (st * C::kStage >> 4) + 2 * k, x_desc + (st * C::kStage >> 4) + 2 * k, idesc, k != 0);
+          umma_commit(&done[st]);
+        }
       }
-      if (failed) drain_mma(&gone);
+      if (!ok) drain_mma(&gone);
     }
   } else if (warp == C::kEpiWarps + 2) {
-    // The blocks' scales, row scale times matrix scale, kScaleSlots blocks ahead.
+    // The blocks' scales, row scale times matrix scale; fetched four blocks before they are stored.
     pdl_wait();
     constexpr int kPer = (BN + 31) / 32;
     const float* ws = p.m.scales + (int64_t)tile * a.kblocks + b0;
-    const float* xs = p.scales + (int64_t)b0 * p.scale_stride + r0;
-    for (int i0 = 0; i0 < nb; i0 += 4) {
-      float v[4][kPer];
+    const float* xs = p.scales + (int64_t)b0 * p.scale_stride + r0 + lane;
+    float sx[4][kPer], sw[4];
+    auto fetch = [&](int j, int i) {
+      sw[j] = i < nb ? ws[i] : 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; j++)
+      for (int c = 0; c < kPer; c++) sx[j][c] = i < nb && c * 32 + lane < valid ? xs[(int64_t)i * p.scale_stride + c * 32] : 0.f;
+    };
 #pragma unroll
-        for (int c = 0; c < kPer; c++) {
-          const int col = c * 32 + lane;
-          v[j][c] = i0 + j < nb && col < valid ? xs[(int64_t)(i0 + j) * p.scale_stride + col] * ws[i0 + j] : 0.f;
-        }
-      bool ok = true;
+    for (int j = 0; j < 4; j++) fetch(j, j);
+    bool ok = true;
+    int st = 0;
+    uint32_t parity = 1;
+    for (int i0 = 0; i0 < nb && ok; i0 += 4) {
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const int i = i0 + j;
-        if (i >= nb || !ok) break;
-        const int slot = i % C::kScaleSlots;
-        if (i >= C::kScaleSlots) ok = role_wait(&sempty[slot], ((i / C::kScaleSlots) - 1) & 1, &failed);
+        if (i0 + j >= nb || !ok) break;
+        ok = role_wait(smem_addr(&read[st]), parity, &failed);
         if (!ok) break;
 #pragma unroll
         for (int c = 0; c < kPer; c++)
-          if (c * 32 + lane < BN) scale_ring[slot * BN + c * 32 + lane] = v[j][c];
+          if (c * 32 + lane < BN) scale_ring[st * BN + c * 32 + lane] = sx[j][c] * sw[j];
+        fetch(j, i0 + j + 4);
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sfull[slot]);
+        if (lane == 0) mbar_arrive(&scaled[st]);
+        if (++st == C::kStages) {
+          st = 0;
+          parity ^= 1;
+        }
       }
-      if (!ok) break;
     }
   } else {
     pdl_wait();
     const int c0 = (warp >> 2) * C::kCpt;
     const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16) + c0;
+    int st = 0;
+    uint32_t parity = 0;
     for (int i = 0; i < nb; i++) {
-      const int slot = i % C::kScaleSlots, buf = i % C::kBufs;
-      if (!role_wait(&sfull[slot], (i / C::kScaleSlots) & 1, &failed)) break;
-      if (!role_wait(&tfull[buf], (i / C::kBufs) & 1, &failed)) break;
+      if (!role_wait(smem_addr(&scaled[st]), parity, &failed) || !role_wait(smem_addr(&done[st]), parity, &failed)) break;
       __syncwarp();
       tc_fence_after();
-      const float4* s4 = reinterpret_cast<const float4*>(scale_ring + slot * BN + c0);
-      uint32_t t[16];
+      const ulonglong2* s2 = reinterpret_cast<const ulonglong2*>(scale_ring + st * BN + c0);
 #pragma unroll
-      for (int c = 0; c < C::kCpt; c += 16) {
-        tmem_ld16_async(trow + buf * BN + c, t);
-        tmem_wait(t);
+      for (int c = 0; c < C::kCpt; c += C::kLd) {
+        uint64_t t[C::kLd / 2];
+        tmem_ld_pairs<C::kLd>(trow + st * BN + c, t);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const float4 s = s4[c / 4 + j];
-          acc[c + 4 * j + 0] = fmaf(__uint_as_float(t[4 * j + 0]), s.x, acc[c + 4 * j + 0]);
-          acc[c + 4 * j + 1] = fmaf(__uint_as_float(t[4 * j + 1]), s.y, acc[c + 4 * j + 1]);
-          acc[c + 4 * j + 2] = fmaf(__uint_as_float(t[4 * j + 2]), s.z, acc[c + 4 * j + 2]);
-          acc[c + 4 * j + 3] = fmaf(__uint_as_float(t[4 * j + 3]), s.w, acc[c + 4 * j + 3]);
+        for (int j = 0; j < C::kLd / 4; j++) {
+          const ulonglong2 s = s2[c / 4 + j];
+          fma_pair(acc[c / 2 + 2 * j], t[2 * j], s.x);
+          fma_pair(acc[c / 2 + 2 * j + 1], t[2 * j + 1], s.y);
         }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&tempty[buf]);
-        mbar_arrive(&sempty[slot]);
+      if (lane == 0) mbar_arrive(&read[st]);
+      if (++st == C::kStages) {
+        st = 0;
+        parity ^= 1;
       }
     }
   }
@@ -234,10 +247,10 @@ __global__ void __launch_bounds__(Thin<BN>::kThreads) f8_thin_kernel(const __gri
 
   const int row_l = (warp & 3) * 32 + lane;
   const int n = tile * kF8Block + row_l;
-  auto put = [&](int c, float y) {  // output (r0 + c, n): consecutive lanes, consecutive columns
+  const float bias = p.m.bias && n < p.m.n ? p.m.bias[n] : 0.f;
+  auto put = [&](int64_t at, float y) {  // consecutive lanes, consecutive columns
     if (n >= p.m.n) return;
-    if (p.m.bias) y = y + p.m.bias[n];
-    const int64_t at = (int64_t)(r0 + c) * p.out_stride + n;
+    if (p.m.bias) y = y + bias;
     if (p.out_bf16)
       static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(y);
     else
@@ -246,32 +259,55 @@ __global__ void __launch_bounds__(Thin<BN>::kThreads) f8_thin_kernel(const __gri
   if (S == 1) {
     if (warp < C::kEpiWarps) {
       const int c0 = (warp >> 2) * C::kCpt;
+      int64_t at = (int64_t)(r0 + c0) * p.out_stride + n;
 #pragma unroll
-      for (int c = 0; c < C::kCpt; c++)
-        if (c0 + c < valid) put(c0 + c, acc[c]);
+      for (int c = 0; c < C::kCpt; c++, at += p.out_stride)
+        if (c0 + c < valid) put(at, c & 1 ? pair_hi(acc[c / 2]) : pair_lo(acc[c / 2]));
     }
   } else {
-    // Every CTA of the cluster is done with its ring: it becomes the exchange [rank][column of the
-    // owner][matrix row]. The owner of column c is rank c / cpr.
-    const int cpr = (valid + S - 1) / S;
+    // Every CTA of the cluster is done with its ring: it becomes the exchange, [rank][group of
+    // kV columns of the owner][matrix row][kV]. Rank o owns the columns [o * cpr, (o + 1) * cpr).
+    constexpr int kV = BN <= 16 ? 1 : 4;
+    const int cpr = ((valid + S - 1) / S + kV - 1) / kV * kV;
     float* recv = reinterpret_cast<float*>(smem);
     cluster_sync();
     if (warp < C::kEpiWarps) {
       const int c0 = (warp >> 2) * C::kCpt;
+      float* mine = recv + ((size_t)rank * cpr * kF8Block + row_l * kV);
+      int owner = c0 / cpr, lc = c0 % cpr;
+      uint32_t to = c0 < valid ? dsmem_addr(mine, owner) : 0;
 #pragma unroll
-      for (int c = 0; c < C::kCpt; c++) {
+      for (int c = 0; c < C::kCpt; c += kV) {
         if (c0 + c >= valid) break;
-        const int owner = (c0 + c) / cpr, lc = (c0 + c) % cpr;
-        dsmem_st(dsmem_addr(recv + ((size_t)rank * cpr + lc) * kF8Block + row_l, owner), acc[c]);
+        if constexpr (kV == 1)
+          dsmem_st(to + lc * kF8Block * 4, c & 1 ? pair_hi(acc[c / 2]) : pair_lo(acc[c / 2]));
+        else
+          dsmem_st4(to + lc * kF8Block * 4, pair_lo(acc[c / 2]), pair_hi(acc[c / 2]), pair_lo(acc[c / 2 + 1]), pair_hi(acc[c / 2 + 1]));
+        lc += kV;
+        if (lc == cpr && c0 + c + kV < valid) {
+          lc = 0;
+          to = dsmem_addr(mine, ++owner);
+        }
       }
     }
     cluster_sync();
     if (warp < C::kEpiWarps) {
       const int mine = min(cpr, valid - rank * cpr);
-      for (int lc = warp >> 2; lc < mine; lc += C::kEpiWarps / 4) {
-        float y = 0.f;
-        for (int q = 0; q < S; q++) y += recv[((size_t)q * cpr + lc) * kF8Block + row_l];
-        put(rank * cpr + lc, y);
+      for (int lc = (warp >> 2) * kV; lc < mine; lc += C::kEpiWarps / 4 * kV) {
+        float y[kV];
+#pragma unroll
+        for (int e = 0; e < kV; e++) y[e] = 0.f;
+#pragma unroll
+        for (int q = 0; q < kMaxSplit; q++) {
+          if (q >= S) break;
+          const float* src = recv + ((size_t)q * cpr + lc) * kF8Block + row_l * kV;
+#pragma unroll
+          for (int e = 0; e < kV; e++) y[e] += src[e];
+        }
+        int64_t at = (int64_t)(r0 + rank * cpr + lc) * p.out_stride + n;
+#pragma unroll
+        for (int e = 0; e < kV; e++, at += p.out_stride)
+          if (lc + e < mine) put(at, y[e]);
       }
     }
   }
@@ -285,25 +321,92 @@ __global__ void __launch_bounds__(Thin<BN>::kThreads) f8_thin_kernel(const __gri
 
 // Bound by the tensor cores and by the operands' way from L2. With the rows as M, a thread of the
 // epilogue holds one row, so a block's scale is one number per thread (no shared-memory reads).
+// Persistent: a CTA takes every gridDim-th tile, and loads and products of the next tile run
+// while one is stored.
 template <int TN>
 struct Wide {
   static constexpr int kEpiWarps = 8;
   // Loader and MMA issuer in a third warpgroup, which for TN = 256 gives registers to the other two
-  // (128 running sums per thread): 384 x 168 at launch, 2 x 128 x 208 + 128 x 72 afterwards.
+  // (128 running sums per thread): 384 x 168 at launch, 2 x 128 x 224 + 128 x 56 afterwards.
   static constexpr bool kShift = TN == 256;
   static constexpr int kThreads = 384;
   static constexpr uint32_t kWBytes = TN * kF8Block;
   static constexpr uint32_t kStage = kTile + kWBytes;
   static constexpr int kStages = (int)(192 * 1024 / kStage);
-  static constexpr int kBufs = 2;
-  static constexpr uint32_t kCols = TN * kBufs;
+  static constexpr int kBufs = TN == 256 ? 2 : 3;
   static constexpr size_t kRing = (size_t)kStages * kStage;
-  static constexpr int kPad = 32 * 9;  // floats per warp: 32 rows x 8 columns, for unaligned outputs
-  static constexpr size_t kSmem = kRing + kEpiWarps * kPad * 4 + 1024;
+  static constexpr uint32_t kPad = 32 * 128;  // bytes per warp: 128 bytes of each of 32 output rows
+  static constexpr size_t kSmem = kRing + kEpiWarps * kPad + 1024;
   static constexpr int kCpt = TN / 2;
   static constexpr int kGroups = TN / 8;  // groups of 8 columns, the unit of the exchange
+  static_assert(kStages % kBufs == 0, "stages and buffers share one unrolled loop");
   static_assert((size_t)(kGroups + kMaxSplit) * 8 * kF8Block * 4 <= kRing, "the exchange reuses the ring");
 };
+
+// Stores chunks of 128 bytes per row (32 f32 or 64 bf16 columns) for the 32 rows a warp's lanes hold.
+// Through shared memory (16-byte pieces permuted by row, so neither side has bank conflicts): a
+// lane's own row would make every store touch 32 lines; this way one store instruction covers
+// whole lines of four rows.
+struct RowStore {
+  const F8GemmParams& p;
+  uint32_t pad;   // this warp's 4 KB of shared memory
+  int lane;
+  int64_t r0;     // the row of lane 0
+  bool aligned;   // rows start on 16 bytes
+
+  // Piece j of this lane's row: 4 f32 or 8 bf16 values of columns n0 + j * 4 (8).
+  __device__ __forceinline__ void piece(int j, uint32_t a, uint32_t b, uint32_t c, uint32_t d) const {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(pad + lane * 128 + ((j ^ (lane & 7)) << 4)), "r"(a),
+                 "r"(b), "r"(c), "r"(d)
+                 : "memory");
+  }
+  __device__ __forceinline__ uint4 at(int row, int j) const {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(pad + row * 128 + ((j ^ (row & 7)) << 4))
+                 : "memory");
+    return v;
+  }
+  // The chunk that starts at column n0, `bytes` (at most 128, for the last columns less) of it.
+  template <class T>
+  __device__ __forceinline__ void out(int n0) const {
+    constexpr int kPer = 16 / sizeof(T);
+    __syncwarp();
+    const int cols = min(128 / (int)sizeof(T), p.m.n - n0);
+    T* base = static_cast<T*>(p.out) + r0 * p.out_stride + n0;
+    if (aligned && cols == 128 / (int)sizeof(T)) {
+      const int j = lane & 7;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const int row = i * 4 + (lane >> 3);
+        const uint4 v = at(row, j);
+        if (r0 + row < p.rows) *reinterpret_cast<uint4*>(base + row * p.out_stride + j * kPer) = v;
+      }
+    } else {
+      const int rows = (int)min((int64_t)32, p.rows - r0);
+      for (int row = 0; row < rows; row++)
+        for (int c = lane; c < cols; c += 32) {
+          const uint32_t from = pad + row * 128 + (((c / kPer) ^ (row & 7)) << 4) + c % kPer * sizeof(T);
+          if constexpr (sizeof(T) == 4) {
+            uint32_t v;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(from) : "memory");
+            reinterpret_cast<uint32_t*>(base)[row * p.out_stride + c] = v;
+          } else {
+            uint16_t v;
+            asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(from) : "memory");
+            reinterpret_cast<uint16_t*>(base)[row * p.out_stride + c] = v;
+          }
+        }
+    }
+    __syncwarp();
+  }
+};
+
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 
 template <int TN>
 __global__ void __launch_bounds__(Wide<TN>::kThreads, 1) f8_wide_kernel(const __grid_constant__ CUtensorMap tm_x,
@@ -311,7 +414,6 @@ __global__ void __launch_bounds__(Wide<TN>::kThreads, 1) f8_wide_kernel(const __
   using C = Wide<TN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* pad = reinterpret_cast<float*>(smem + C::kRing);
   __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages], tfull[C::kBufs], tempty[C::kBufs], gone;
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
@@ -336,7 +438,7 @@ __global__ void __launch_bounds__(Wide<TN>::kThreads, 1) f8_wide_kernel(const __
     failed = 0;
     fence_mbar_init();
   }
-  if (warp == C::kEpiWarps + 1) tmem_alloc(&tmem_slot, C::kCols);
+  if (warp == C::kEpiWarps + 1) tmem_alloc(&tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -344,41 +446,58 @@ __global__ void __launch_bounds__(Wide<TN>::kThreads, 1) f8_wide_kernel(const __
   pdl_wait();
 
   if (warp >= C::kEpiWarps) {
-    if (C::kShift) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (C::kShift) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == C::kEpiWarps && lane == 0) {
-      int it = 0;
-      for (int tile = first; tile < total && !failed; tile += stride) {
-        const int nt = tile % a.ntiles, rt = tile / a.ntiles;
-        const int wt = nt * kTiles, have = min(kTiles, p.m.tiles() - wt);
-        for (int b = b0; b < b0 + nb; b++, it++) {
-          const int st = it % C::kStages;
-          if (it >= C::kStages && !role_wait(&empty[st], ((it / C::kStages) - 1) & 1, &failed)) break;
-          mbar_expect_tx(&full[st], kTile * (1 + have));
+      int issued = 0, st = 0;
+      uint32_t parity = 1;
+      bool ok = true;
+      for (int tile = first; tile < total && ok; tile += stride) {
+        const int nt = tile % a.ntiles, row = tile / a.ntiles * kF8Block;
+        const int have = min(kTiles, p.m.tiles() - nt * kTiles);
+        const uint8_t* w = p.m.w + ((int64_t)nt * kTiles * a.kblocks + b0) * kF8TileBytes;
+        const int64_t next = (int64_t)a.kblocks * kF8TileBytes;  // the same block of the next 128 matrix rows
+        for (int b = b0; b < b0 + nb; b++, issued++, w += kF8TileBytes) {
+          ok = role_wait(smem_addr(&empty[st]), parity, &failed);
+          if (!ok) break;
+          uint64_t* bar = &full[st];
           uint8_t* at = smem + (size_t)st * C::kStage;
-          tma_load_2d(at, &tm_x, b * kF8Block, rt * kF8Block, &full[st]);
-          for (int j = 0; j < have; j++)
-            bulk_g2s(at + kTile * (1 + j), p.m.w + ((int64_t)(wt + j) * a.kblocks + b) * kF8TileBytes, kTile, &full[st]);
+          mbar_expect_tx(bar, kTile * (1 + have));
+          tma_load_2d(at, &tm_x, b * kF8Block, row, bar);
+          bulk_g2s(at + kTile, w, kTile, bar);
+          if (kTiles > 1 && have > 1) bulk_g2s(at + 2 * kTile, w + next, kTile, bar);
+          if (++st == C::kStages) {
+            st = 0;
+            parity ^= 1;
+          }
         }
       }
       pdl_launch();
-      drain_loads(full, it, C::kStages);
+      drain_loads(full, issued, C::kStages);
     } else if (warp == C::kEpiWarps + 1 && lane == 0) {
+      // Tiles make no difference here: every block is a product of its own.
       constexpr uint32_t idesc = idesc_e4m3(kF8Block, TN);
-      int it = 0;
-      for (int tile = first; tile < total && !failed; tile += stride)
-        for (int b = 0; b < nb; b++, it++) {
-          const int st = it % C::kStages, buf = it % C::kBufs;
-          if (it >= C::kBufs && !role_wait(&tempty[buf], ((it / C::kBufs) - 1) & 1, &failed)) break;
-          if (!role_wait(&full[st], (it / C::kStages) & 1, &failed)) break;
+      constexpr int kTurns = C::kStages / C::kBufs;  // of the buffers per pass over the stages
+      const uint32_t full_at = smem_addr(full), tempty_at = smem_addr(tempty);
+      const uint64_t x_desc = sw128_desc(smem_addr(smem)), w_desc = sw128_desc(smem_addr(smem) + kTile);
+      uint32_t pass = 0;
+      bool ok = true;
+      for (int left = (total - first + stride - 1) / stride * nb; left > 0 && ok; left -= C::kStages, pass++) {
+#pragma unroll
+        for (int st = 0; st < C::kStages; st++) {
+          if (st >= left || !ok) break;
+          constexpr int kB = C::kBufs;
+          ok = role_wait(tempty_at + 8 * (st % kB), (pass * kTurns + st / kB + 1) & 1, &failed) &&
+               role_wait(full_at + 8 * st, pass & 1, &failed);
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t xa = smem_addr(smem + (size_t)st * C::kStage), wa = xa + kTile;
 #pragma unroll
           for (int k = 0; k < 4; k++)
-            umma_f8(tmem + buf * TN, sw128_desc(xa + k * 32), sw128_desc(wa + k * 32), idesc, k != 0);
+            umma_f8(tmem + st % kB * TN, x_desc + (st * C::kStage >> 4) + 2 * k, w_desc + (st * C::kStage >> 4) + 2 * k, idesc, k != 0);
           umma_commit(&empty[st]);
-          umma_commit(&tfull[buf]);
+          umma_commit(&tfull[st % kB]);
         }
-      if (failed) drain_mma(&gone);
+      }
+      if (!ok) drain_mma(&gone);
     }
     if (S > 1) {
       __syncwarp();
@@ -386,103 +505,95 @@ __global__ void __launch_bounds__(Wide<TN>::kThreads, 1) f8_wide_kernel(const __
       cluster_sync();
     }
   } else {
-    if (C::kShift) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    if (C::kShift) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int half = warp >> 2, row_l = (warp & 3) * 32 + lane;
     const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * C::kCpt;
     const bool bf16 = p.out_bf16;
-    // 16-byte stores: a row's groups of 8 columns start on 16 bytes.
-    const bool aligned = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.out_stride % (bf16 ? 8 : 4) == 0;
-    float* my = pad + warp * C::kPad;
-    // Columns [n, n + 8) of row r, held by the warp's lanes for 32 consecutive rows.
-    auto put8 = [&](int64_t r, int n, float (&y)[8]) {
-      if (n >= p.m.n) return;
-      if (p.m.bias) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) y[j] = y[j] + (n + j < p.m.n ? p.m.bias[n + j] : 0.f);
-      }
-      if (aligned && n + 8 <= p.m.n) {
-        if (r >= p.rows) return;
-        if (bf16) {
-          __nv_bfloat162 h[4];
-#pragma unroll
-          for (int j = 0; j < 4; j++) h[j] = __floats2bfloat162_rn(y[2 * j], y[2 * j + 1]);
-          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + r * p.out_stride + n) = *reinterpret_cast<uint4*>(h);
-        } else {
-          float4* o = reinterpret_cast<float4*>(static_cast<float*>(p.out) + r * p.out_stride + n);
-          o[0] = make_float4(y[0], y[1], y[2], y[3]);
-          o[1] = make_float4(y[4], y[5], y[6], y[7]);
-        }
-        return;
-      }
-#pragma unroll
-      for (int j = 0; j < 8; j++) my[lane * 9 + j] = y[j];
-      __syncwarp();
-      const int c = lane & 7;
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const int rr = j * 4 + (lane >> 3);
-        const int64_t at = r - lane + rr;
-        if (at < p.rows && n + c < p.m.n) {
-          if (bf16)
-            static_cast<__nv_bfloat16*>(p.out)[at * p.out_stride + n + c] = __float2bfloat16_rn(my[rr * 9 + c]);
-          else
-            static_cast<float*>(p.out)[at * p.out_stride + n + c] = my[rr * 9 + c];
-        }
-      }
-      __syncwarp();
-    };
-    int it = 0;
+    RowStore rs{p, smem_addr(smem + C::kRing) + warp * C::kPad, lane, 0,
+                reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.out_stride % (bf16 ? 8 : 4) == 0};
+    auto bias_at = [&](int n) { return p.m.bias && n < p.m.n ? p.m.bias[n] : 0.f; };
+    int buf = 0;
+    uint32_t parity = 0;
     for (int tile = first; tile < total; tile += stride) {
       const int nt = tile % a.ntiles, rt = tile / a.ntiles;
       const int64_t r = (int64_t)rt * kF8Block + row_l;
+      rs.r0 = r - lane;
       const int wt = nt * kTiles + (kTiles > 1 ? half : 0);
       const bool live = r < p.rows && wt < p.m.tiles();
       const float* xs = p.scales + (int64_t)b0 * p.scale_stride + (live ? r : 0);
       const float* ws = p.m.scales + (int64_t)(live ? wt : 0) * a.kblocks + b0;
-      auto scale_at = [&](int b) { return live && b < nb ? xs[(int64_t)b * p.scale_stride] * ws[b] : 0.f; };
-      float acc[C::kCpt];
+      uint64_t acc[C::kCpt / 2];
 #pragma unroll
-      for (int i = 0; i < C::kCpt; i++) acc[i] = 0.f;
-      float s[4];
+      for (int i = 0; i < C::kCpt / 2; i++) acc[i] = 0;
+      // The blocks' scales, four blocks ahead; multiplied where they are used, since a product here
+      // would wait for its loads.
+      float sx[4], sw[4];
+      auto fetch = [&](int j, int b) {
+        sx[j] = live && b < nb ? *xs : 0.f;
+        sw[j] = live && b < nb ? ws[b] : 0.f;
+        xs += p.scale_stride;
+      };
 #pragma unroll
-      for (int j = 0; j < 4; j++) s[j] = scale_at(j);
+      for (int j = 0; j < 4; j++) fetch(j, j);
       bool ok = true;
       for (int b1 = 0; b1 < nb && ok; b1 += 4) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           if (b1 + j >= nb || !ok) break;
-          const int buf = it % C::kBufs;
-          ok = role_wait(&tfull[buf], (it / C::kBufs) & 1, &failed);
+          ok = role_wait(smem_addr(&tfull[buf]), parity, &failed);
           if (!ok) break;
           __syncwarp();
           tc_fence_after();
-          const float sc = s[j];
-          s[j] = scale_at(b1 + j + 4);
-          uint32_t t[16];
+          const float sc = sx[j] * sw[j];
+          const uint64_t sc2 = pair_of(sc, sc);
+          fetch(j, b1 + j + 4);
 #pragma unroll
           for (int c = 0; c < C::kCpt; c += 16) {
-            tmem_ld16_async(trow + buf * TN + c, t);
-            tmem_wait(t);
+            uint64_t t[8];
+            tmem_ld_pairs<16>(trow + buf * TN + c, t);
 #pragma unroll
-            for (int e = 0; e < 16; e++) acc[c + e] = fmaf(__uint_as_float(t[e]), sc, acc[c + e]);
+            for (int e = 0; e < 8; e++) fma_pair(acc[c / 2 + e], t[e], sc2);
           }
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&tempty[buf]);
-          it++;
+          if (++buf == C::kBufs) {
+            buf = 0;
+            parity ^= 1;
+          }
         }
       }
       if (S == 1) {
-        if (ok) {
+        if (!ok) break;
+        const int n0 = nt * TN + half * C::kCpt;
+        if (p.m.bias) {
 #pragma unroll
-          for (int c = 0; c < C::kCpt; c += 8) {
-            float y[8];
+          for (int c = 0; c < C::kCpt; c += 2)
+            acc[c / 2] = pair_of(pair_lo(acc[c / 2]) + bias_at(n0 + c), pair_hi(acc[c / 2]) + bias_at(n0 + c + 1));
+        }
+        if (bf16) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) y[e] = acc[c + e];
-            put8(r, nt * TN + half * C::kCpt + c, y);
+          for (int c = 0; c < C::kCpt; c += 64) {
+            if (n0 + c >= p.m.n) break;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+              const uint64_t* v = acc + c / 2 + 4 * j;
+              rs.piece(j, bf16_pair(pair_lo(v[0]), pair_hi(v[0])), bf16_pair(pair_lo(v[1]), pair_hi(v[1])),
+                       bf16_pair(pair_lo(v[2]), pair_hi(v[2])), bf16_pair(pair_lo(v[3]), pair_hi(v[3])));
+            }
+            rs.out<__nv_bfloat16>(n0 + c);
           }
         } else {
-          break;
+#pragma unroll
+          for (int c = 0; c < C::kCpt; c += 32) {
+            if (n0 + c >= p.m.n) break;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+              const uint64_t* v = acc + c / 2 + 2 * j;
+              rs.piece(j, (uint32_t)v[0], (uint32_t)(v[0] >> 32), (uint32_t)v[1], (uint32_t)(v[1] >> 32));
+            }
+            rs.out<float>(n0 + c);
+          }
         }
       } else {
         // One tile per cluster: its CTAs exchange their sums through the rings they are done
@@ -499,20 +610,48 @@ __global__ void __launch_bounds__(Wide<TN>::kThreads, 1) f8_wide_kernel(const __
           while (g >= (owner + 1) * G / S) owner++;
           const int lg = g - owner * G / S;
           const uint32_t at = dsmem_addr(recv + (((size_t)rank * most + lg) * 2 * kF8Block + row_l) * 4, owner);
-          dsmem_st4(at, acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
-          dsmem_st4(at + kF8Block * 16, acc[c + 4], acc[c + 5], acc[c + 6], acc[c + 7]);
+          const uint64_t* v = acc + c / 2;
+          dsmem_st4(at, pair_lo(v[0]), pair_hi(v[0]), pair_lo(v[1]), pair_hi(v[1]));
+          dsmem_st4(at + kF8Block * 16, pair_lo(v[2]), pair_hi(v[2]), pair_lo(v[3]), pair_hi(v[3]));
         }
         cluster_sync();
         const int g0 = rank * G / S, g1 = (rank + 1) * G / S;
         for (int g = g0 + half; g < g1; g += 2) {
+          const int n = nt * TN + g * 8;
+          if (n >= p.m.n) break;
           float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          for (int q = 0; q < S; q++) {
+#pragma unroll
+          for (int q = 0; q < kMaxSplit; q++) {
+            if (q >= S) break;
             const float4* src = reinterpret_cast<const float4*>(recv) + ((size_t)q * most + (g - g0)) * 2 * kF8Block + row_l;
             const float4 u = src[0], v = src[kF8Block];
             y[0] += u.x; y[1] += u.y; y[2] += u.z; y[3] += u.w;
             y[4] += v.x; y[5] += v.y; y[6] += v.z; y[7] += v.w;
           }
-          put8(r, nt * TN + g * 8, y);
+          if (r >= p.rows) continue;
+          const bool whole = rs.aligned && n + 8 <= p.m.n;
+          if (p.m.bias) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] = y[e] + bias_at(n + e);
+          }
+          if (bf16) {
+            __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + r * p.out_stride + n;
+            if (whole)
+              *reinterpret_cast<uint4*>(o) = make_uint4(bf16_pair(y[0], y[1]), bf16_pair(y[2], y[3]), bf16_pair(y[4], y[5]), bf16_pair(y[6], y[7]));
+            else
+#pragma unroll
+              for (int e = 0; e < 8; e++)
+                if (n + e < p.m.n) o[e] = __float2bfloat16_rn(y[e]);
+          } else {
+            float* o = static_cast<float*>(p.out) + r * p.out_stride + n;
+            if (whole) {
+              reinterpret_cast<float4*>(o)[0] = make_float4(y[0], y[1], y[2], y[3]);
+              reinterpret_cast<float4*>(o)[1] = make_float4(y[4], y[5], y[6], y[7]);
+            } else
+#pragma unroll
+              for (int e = 0; e < 8; e++)
+                if (n + e < p.m.n) o[e] = y[e];
+          }
         }
       }
     }
@@ -520,7 +659,7 @@ __global__ void __launch_bounds__(Wide<TN>::kThreads, 1) f8_wide_kernel(const __
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && failed && p.err) atomicExch(p.err, 2);
-  if (warp == C::kEpiWarps + 1) tmem_free(tmem, C::kCols);
+  if (warp == C::kEpiWarps + 1) tmem_free(tmem, 512);
 }
 
 // ---- host side ----------------------------------------------------------------------------

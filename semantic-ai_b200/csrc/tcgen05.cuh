@@ -73,24 +73,57 @@ __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t a, uint64_t b,
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// 16 consecutive columns of this thread's TMEM lane, in flight until tmem_wait(v).
-__device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t (&r)[16]) {
+// N consecutive columns of this thread's TMEM lane, as N / 2 pairs (the lower column in the lower
+// half), waited for.
+template <int N>
+__device__ __forceinline__ void tmem_ld_pairs(uint32_t taddr, uint64_t (&v)[N / 2]);
+template <>
+__device__ __forceinline__ void tmem_ld_pairs<16>(uint32_t taddr, uint64_t (&v)[8]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-      "%11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
+      "{\n\t.reg .b32 a<16>;\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {"
+      "a0, a1, a2, a3, a4, a5, a6, a7, a8, a9, a10, a11, a12, a13, a14, a15}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;\n\t"
+      "mov.b64 %0, {a0, a1};\n\tmov.b64 %1, {a2, a3};\n\t"
+      "mov.b64 %2, {a4, a5};\n\tmov.b64 %3, {a6, a7};\n\t"
+      "mov.b64 %4, {a8, a9};\n\tmov.b64 %5, {a10, a11};\n\t"
+      "mov.b64 %6, {a12, a13};\n\tmov.b64 %7, {a14, a15};\n\t}"
+      : "=l"(v[0]), "=l"(v[1]), "=l"(v[2]), "=l"(v[3]), "=l"(v[4]), "=l"(v[5]), "=l"(v[6]), "=l"(v[7])
+      : "r"(taddr)
+      : "memory");
 }
-// Waits for this thread's TMEM loads; r passes through, so that its readers stay behind the wait.
-__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-               :
-               : "memory");
+template <>
+__device__ __forceinline__ void tmem_ld_pairs<32>(uint32_t taddr, uint64_t (&v)[16]) {
+  asm volatile(
+      "{\n\t.reg .b32 a<32>;\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+      "a0, a1, a2, a3, a4, a5, a6, a7, a8, a9, a10, a11, a12, a13, a14, a15, "
+      "a16, a17, a18, a19, a20, a21, a22, a23, a24, a25, a26, a27, a28, a29, a30, a31}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;\n\t"
+      "mov.b64 %0, {a0, a1};\n\tmov.b64 %1, {a2, a3};\n\t"
+      "mov.b64 %2, {a4, a5};\n\tmov.b64 %3, {a6, a7};\n\t"
+      "mov.b64 %4, {a8, a9};\n\tmov.b64 %5, {a10, a11};\n\t"
+      "mov.b64 %6, {a12, a13};\n\tmov.b64 %7, {a14, a15};\n\t"
+      "mov.b64 %8, {a16, a17};\n\tmov.b64 %9, {a18, a19};\n\t"
+      "mov.b64 %10, {a20, a21};\n\tmov.b64 %11, {a22, a23};\n\t"
+      "mov.b64 %12, {a24, a25};\n\tmov.b64 %13, {a26, a27};\n\t"
+      "mov.b64 %14, {a28, a29};\n\tmov.b64 %15, {a30, a31};\n\t}"
+      : "=l"(v[0]), "=l"(v[1]), "=l"(v[2]), "=l"(v[3]), "=l"(v[4]), "=l"(v[5]), "=l"(v[6]), "=l"(v[7]),
+        "=l"(v[8]), "=l"(v[9]), "=l"(v[10]), "=l"(v[11]), "=l"(v[12]), "=l"(v[13]), "=l"(v[14]), "=l"(v[15])
+      : "r"(taddr)
+      : "memory");
 }
+// Pairs of f32: both products and sums in one instruction.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void fma_pair(uint64_t& acc, uint64_t a, uint64_t b) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
+}
+__device__ __forceinline__ float pair_lo(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float pair_hi(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t columns) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(slot)), "r"(columns)
                : "memory");
