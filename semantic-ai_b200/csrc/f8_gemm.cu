@@ -41,9 +41,11 @@ struct F8Args {
   int rtiles;        // tiles along the rows
 };
 
-// The MMA issuer's and the loader's loops are single threads, a block of them has to take less than
-// the block's product (512 clocks for 128 x 256), so they keep shared-memory addresses and
-// descriptors in registers and count stages instead of dividing.
+// A block of the MMA issuer's and the loader's loops has to take less than the block's product (512
+// clocks for 128 x 256). Their warps run the loops as a whole and elect a lane for the copies and
+// products only, so that control flow, waits and addresses stay warp-uniform: a block of four
+// products, two commits and two ready waits takes 374 clocks of issue this way and 588 in a
+// single-lane branch. Stages are counted, not divided.
 
 // A role's bounded wait; a wait that ran out marks the CTA as failed.
 __device__ __forceinline__ bool role_wait(uint32_t bar, uint32_t parity, int* failed) {
@@ -59,35 +61,34 @@ __device__ __forceinline__ void drain_loads(uint64_t* full, int issued, int stag
   for (int i = issued > stages ? issued - stages : 0; i < issued; i++) mbar_wait(&full[i % stages], (i / stages) & 1);
 }
 // The MMA issuer's end after a wait that ran out: the products it has issued are done.
-__device__ __forceinline__ void drain_mma(uint64_t* bar) {
-  umma_commit(bar);
+__device__ __forceinline__ void drain_mma(uint64_t* bar, bool lead) {
+  if (lead) umma_commit(bar);
+  __syncwarp();
   mbar_wait(bar, 0);
 }
 
 // ---- few rows: matrix rows are the MMA's M, up to BN rows its N ------------------------------
 
 // Bound by the weights' bytes: every CTA keeps a ring of about 100 KB of loads in flight, two
-// CTAs per SM (one with 192 KB for 128 rows). A stage of the ring, its TMEM buffer and its scales
+// CTAs per SM. A stage of the ring, its TMEM buffer and its scales
 // share one index and one phase: `full` (loaded), `done` (multiplied: the stage may be loaded
 // again, the buffer read), `read` (the epilogue is through with buffer and scales).
 template <int BN>
 struct Thin {
-  static constexpr int kEpiWarps = BN <= 64 ? 4 : 8;
+  static constexpr int kEpiWarps = 4;
   static constexpr int kThreads = (kEpiWarps + 3) * 32;  // + loader, MMA issuer, scales
   static constexpr uint32_t kXBytes = BN * kF8Block;
   static constexpr uint32_t kStage = kTile + kXBytes;
-  static constexpr int kStages = BN == 16 ? 6 : BN == 32 ? 5 : BN == 64 ? 4 : 4;
-  static constexpr uint32_t kCols = BN == 16 ? 128 : BN == 32 ? 256 : BN == 64 ? 256 : 512;
+  static constexpr int kStages = BN == 16 ? 6 : 5;
+  static constexpr uint32_t kCols = BN == 16 ? 128 : 256;
   static constexpr size_t kRing = (size_t)kStages * kStage;
   static constexpr size_t kSmem = kRing + kStages * BN * 4 + 1024;
-  static constexpr int kCpt = BN / (kEpiWarps / 4);  // columns (rows of x) per epilogue thread
-  static constexpr int kLd = kCpt < 32 ? 16 : 32;    // columns per TMEM load
   static_assert(kStages * BN <= (int)kCols, "a TMEM buffer per stage");
   static_assert((size_t)(BN + 4 * kMaxSplit) * kF8Block * 4 <= kRing, "the exchange reuses the ring");
 };
 
 template <int BN>
-__global__ void __launch_bounds__(Thin<BN>::kThreads, BN <= 64 ? 2 : 1)
+__global__ void __launch_bounds__(Thin<BN>::kThreads, 2)
     f8_thin_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ F8Args a) {
   using C = Thin<BN>;
   extern __shared__ uint8_t smem_raw[];
@@ -97,7 +98,7 @@ __global__ void __launch_bounds__(Thin<BN>::kThreads, BN <= 64 ? 2 : 1)
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
   const F8GemmParams& p = a.p;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int S = a.split;
   const int rank = S > 1 ? (int)cluster_rank() : 0;
   const int tile = blockIdx.x / S;
@@ -105,9 +106,20 @@ __global__ void __launch_bounds__(Thin<BN>::kThreads, BN <= 64 ? 2 : 1)
   const int b0 = (int)((int64_t)rank * a.kblocks / S), nb = (int)((int64_t)(rank + 1) * a.kblocks / S) - b0;
   const int valid = (int)(p.rows - r0 < BN ? p.rows - r0 : BN);
 
+  if (S > 1) cluster_arrive();  // waited for before the exchange: every CTA of the cluster runs
+  const uint8_t* w = p.m.w + ((int64_t)tile * a.kblocks + b0) * kF8TileBytes;
+  const int pre = nb < C::kStages ? nb : C::kStages;
+  if (tid == C::kEpiWarps * 32) {
+    // The weights do not depend on the kernel before, nor on the rest of the setup.
+    for (int i = 0; i < C::kStages; i++) mbar_init(&full[i], 1);
+    fence_mbar_init();
+    for (int i = 0; i < pre; i++) {
+      mbar_expect_tx(&full[i], C::kStage);
+      bulk_g2s(smem + (size_t)i * C::kStage, w + i * kF8TileBytes, kTile, &full[i]);
+    }
+  }
   if (tid == 0) {
     for (int i = 0; i < C::kStages; i++) {
-      mbar_init(&full[i], 1);
       mbar_init(&done[i], 1);
       mbar_init(&read[i], C::kEpiWarps);
       mbar_init(&scaled[i], 1);
@@ -122,63 +134,61 @@ __global__ void __launch_bounds__(Thin<BN>::kThreads, BN <= 64 ? 2 : 1)
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  uint64_t acc[C::kCpt / 2];
+  uint64_t acc[BN / 2];
 #pragma unroll
-  for (int i = 0; i < C::kCpt / 2; i++) acc[i] = 0;
+  for (int i = 0; i < BN / 2; i++) acc[i] = 0;
 
   if (warp == C::kEpiWarps) {
-    if (lane == 0) {
-      // The weights do not depend on the kernel before: their first stages go out before the wait.
-      const uint8_t* w = p.m.w + ((int64_t)tile * a.kblocks + b0) * kF8TileBytes;
-      const int pre = nb < C::kStages ? nb : C::kStages;
-      for (int i = 0; i < pre; i++) {
-        mbar_expect_tx(&full[i], C::kStage);
-        bulk_g2s(smem + (size_t)i * C::kStage, w + i * kF8TileBytes, kTile, &full[i]);
-      }
-      pdl_wait();
+    const bool lead = elect_one();
+    pdl_wait();
+    if (lead)
       for (int i = 0; i < pre; i++)
         tma_load_2d(smem + (size_t)i * C::kStage + kTile, &tm_x, (b0 + i) * kF8Block, r0, &full[i]);
-      w += (int64_t)pre * kF8TileBytes;
-      int i = pre, st = 0;
-      uint32_t parity = 0;
-      for (; i < nb; i++) {
-        if (!role_wait(smem_addr(&done[st]), parity, &failed)) break;
+    w += (int64_t)pre * kF8TileBytes;
+    int i = pre, st = 0;
+    uint32_t parity = 0;
+    for (; i < nb; i++) {
+      if (!role_wait(smem_addr(&done[st]), parity, &failed)) break;
+      if (lead) {
         mbar_expect_tx(&full[st], C::kStage);
         bulk_g2s(smem + (size_t)st * C::kStage, w, kTile, &full[st]);
         tma_load_2d(smem + (size_t)st * C::kStage + kTile, &tm_x, (b0 + i) * kF8Block, r0, &full[st]);
-        w += kF8TileBytes;
-        if (++st == C::kStages) {
-          st = 0;
-          parity ^= 1;
-        }
       }
-      pdl_launch();
-      drain_loads(full, i, C::kStages);
+      __syncwarp();
+      w += kF8TileBytes;
+      if (++st == C::kStages) {
+        st = 0;
+        parity ^= 1;
+      }
     }
+    pdl_launch();
+    drain_loads(full, i, C::kStages);
   } else if (warp == C::kEpiWarps + 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = idesc_e4m3(kF8Block, BN);
-      const uint32_t full_at = smem_addr(full), read_at = smem_addr(read);
-      const uint64_t w_desc = sw128_desc(smem_addr(smem)), x_desc = sw128_desc(smem_addr(smem) + kTile);
-      uint32_t parity = 0;
-      bool ok = true;
-      for (int left = nb; left > 0 && ok; left -= C::kStages, parity ^= 1) {
+    constexpr uint32_t idesc = idesc_e4m3(kF8Block, BN);
+    const bool lead = elect_one();
+    const uint32_t full_at = smem_addr(full), read_at = smem_addr(read);
+    const uint64_t w_desc = sw128_desc(smem_addr(smem)), x_desc = sw128_desc(smem_addr(smem) + kTile);
+    uint32_t parity = 0;
+    bool ok = true;
+    for (int left = nb; left > 0 && ok; left -= C::kStages, parity ^= 1) {
 #pragma unroll
-        for (int st = 0; st < C::kStages; st++) {
-          if (st >= left || !ok) break;
-          ok = role_wait(read_at + 8 * st, parity ^ 1, &failed) && role_wait(full_at + 8 * st, parity, &failed);
-          if (!ok) break;
-          tc_fence_after();
+      for (int st = 0; st < C::kStages; st++) {
+        if (st >= left || !ok) break;
+        ok = role_wait(read_at + 8 * st, parity ^ 1, &failed) && role_wait(full_at + 8 * st, parity, &failed);
+        if (!ok) break;
+        tc_fence_after();
+        if (lead) {
 #pragma unroll
           for (int k = 0; k < 4; k++)
             umma_f8(tmem + st * BN, w_desc + (st * C::kStage >> 4) + 2 * k, x_desc + (st * C::kStage >> 4) + 2 * k, idesc, k != 0);
           umma_commit(&done[st]);
         }
+        __syncwarp();
       }
-      if (!ok) drain_mma(&gone);
     }
+    if (!ok) drain_mma(&gone, lead);
   } else if (warp == C::kEpiWarps + 2) {
-    // The blocks' scales, row scale times matrix scale; fetched four blocks before they are stored.
+    // The blocks' scales, row scale times matrix scale; fetched four at a time.
     pdl_wait();
     constexpr int kPer = (BN + 31) / 32;
     const float* ws = p.m.scales + (int64_t)tile * a.kblocks + b0;
@@ -203,7 +213,6 @@ __global__ void __launch_bounds__(Thin<BN>::kThreads, BN <= 64 ? 2 : 1)
 #pragma unroll
         for (int c = 0; c < kPer; c++)
           if (c * 32 + lane < BN) scale_ring[st * BN + c * 32 + lane] = sx[j][c] * sw[j];
-        fetch(j, i0 + j + 4);
         __syncwarp();
         if (lane == 0) mbar_arrive(&scaled[st]);
         if (++st == C::kStages) {
@@ -211,28 +220,27 @@ __global__ void __launch_bounds__(Thin<BN>::kThreads, BN <= 64 ? 2 : 1)
           parity ^= 1;
         }
       }
+      // Not between the arrivals: each would wait for the loads in flight.
+#pragma unroll
+      for (int j = 0; j < 4; j++) fetch(j, i0 + j + 4);
     }
   } else {
     pdl_wait();
-    const int c0 = (warp >> 2) * C::kCpt;
-    const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16) + c0;
+    const uint32_t trow = tmem + ((uint32_t)(warp * 32) << 16);
     int st = 0;
     uint32_t parity = 0;
     for (int i = 0; i < nb; i++) {
       if (!role_wait(smem_addr(&scaled[st]), parity, &failed) || !role_wait(smem_addr(&done[st]), parity, &failed)) break;
       __syncwarp();
       tc_fence_after();
-      const ulonglong2* s2 = reinterpret_cast<const ulonglong2*>(scale_ring + st * BN + c0);
+      const ulonglong2* s2 = reinterpret_cast<const ulonglong2*>(scale_ring + st * BN);
+      uint64_t t[BN / 2];
+      tmem_ld_pairs<BN>(trow + st * BN, t);
 #pragma unroll
-      for (int c = 0; c < C::kCpt; c += C::kLd) {
-        uint64_t t[C::kLd / 2];
-        tmem_ld_pairs<C::kLd>(trow + st * BN + c, t);
-#pragma unroll
-        for (int j = 0; j < C::kLd / 4; j++) {
-          const ulonglong2 s = s2[c / 4 + j];
-          fma_pair(acc[c / 2 + 2 * j], t[2 * j], s.x);
-          fma_pair(acc[c / 2 + 2 * j + 1], t[2 * j + 1], s.y);
-        }
+      for (int j = 0; j < BN / 4; j++) {
+        const ulonglong2 s = s2[j];
+        fma_pair(acc[2 * j], t[2 * j], s.x);
+        fma_pair(acc[2 * j + 1], t[2 * j + 1], s.y);
       }
       tc_fence_before();
       __syncwarp();
@@ -258,11 +266,10 @@ __global__ void __launch_bounds__(Thin<BN>::kThreads, BN <= 64 ? 2 : 1)
   };
   if (S == 1) {
     if (warp < C::kEpiWarps) {
-      const int c0 = (warp >> 2) * C::kCpt;
-      int64_t at = (int64_t)(r0 + c0) * p.out_stride + n;
+      int64_t at = (int64_t)r0 * p.out_stride + n;
 #pragma unroll
-      for (int c = 0; c < C::kCpt; c++, at += p.out_stride)
-        if (c0 + c < valid) put(at, c & 1 ? pair_hi(acc[c / 2]) : pair_lo(acc[c / 2]));
+      for (int c = 0; c < BN; c++, at += p.out_stride)
+        if (c < valid) put(at, c & 1 ? pair_hi(acc[c / 2]) : pair_lo(acc[c / 2]));
     }
   } else {
     // Every CTA of the cluster is done with its ring: it becomes the exchange, [rank][group of
@@ -270,21 +277,21 @@ __global__ void __launch_bounds__(Thin<BN>::kThreads, BN <= 64 ? 2 : 1)
     constexpr int kV = BN <= 16 ? 1 : 4;
     const int cpr = ((valid + S - 1) / S + kV - 1) / kV * kV;
     float* recv = reinterpret_cast<float*>(smem);
+    cluster_wait();
     cluster_sync();
     if (warp < C::kEpiWarps) {
-      const int c0 = (warp >> 2) * C::kCpt;
       float* mine = recv + ((size_t)rank * cpr * kF8Block + row_l * kV);
-      int owner = c0 / cpr, lc = c0 % cpr;
-      uint32_t to = c0 < valid ? dsmem_addr(mine, owner) : 0;
+      int owner = 0, lc = 0;
+      uint32_t to = dsmem_addr(mine, owner);
 #pragma unroll
-      for (int c = 0; c < C::kCpt; c += kV) {
-        if (c0 + c >= valid) break;
+      for (int c = 0; c < BN; c += kV) {
+        if (c >= valid) break;
         if constexpr (kV == 1)
           dsmem_st(to + lc * kF8Block * 4, c & 1 ? pair_hi(acc[c / 2]) : pair_lo(acc[c / 2]));
         else
           dsmem_st4(to + lc * kF8Block * 4, pair_lo(acc[c / 2]), pair_hi(acc[c / 2]), pair_lo(acc[c / 2 + 1]), pair_hi(acc[c / 2 + 1]));
         lc += kV;
-        if (lc == cpr && c0 + c + kV < valid) {
+        if (lc == cpr && c + kV < valid) {
           lc = 0;
           to = dsmem_addr(mine, ++owner);
         }
@@ -293,7 +300,7 @@ __global__ void __launch_bounds__(Thin<BN>::kThreads, BN <= 64 ? 2 : 1)
     cluster_sync();
     if (warp < C::kEpiWarps) {
       const int mine = min(cpr, valid - rank * cpr);
-      for (int lc = (warp >> 2) * kV; lc < mine; lc += C::kEpiWarps / 4 * kV) {
+      for (int lc = 0; lc < mine; lc += kV) {
         float y[kV];
 #pragma unroll
         for (int e = 0; e < kV; e++) y[e] = 0.f;
@@ -317,87 +324,59 @@ __global__ void __launch_bounds__(Thin<BN>::kThreads, BN <= 64 ? 2 : 1)
   if (warp == C::kEpiWarps + 1) tmem_free(tmem, C::kCols);
 }
 
-// ---- many rows: the rows are the MMA's M, TN matrix rows its N --------------------------------
-
-// Bound by the tensor cores and by the operands' way from L2. With the rows as M, a thread of the
-// epilogue holds one row, so a block's scale is one number per thread (no shared-memory reads).
-// Persistent: a CTA takes every gridDim-th tile, and loads and products of the next tile run
-// while one is stored.
-template <int TN>
-struct Wide {
-  static constexpr int kEpiWarps = 8;
-  // Loader and MMA issuer in a third warpgroup, which for TN = 256 gives registers to the other two
-  // (128 running sums per thread): 384 x 168 at launch, 2 x 128 x 224 + 128 x 56 afterwards.
-  static constexpr bool kShift = TN == 256;
-  static constexpr int kThreads = 384;
-  static constexpr uint32_t kWBytes = TN * kF8Block;
-  static constexpr uint32_t kStage = kTile + kWBytes;
-  static constexpr int kStages = (int)(192 * 1024 / kStage);
-  static constexpr int kBufs = TN == 256 ? 2 : 3;
-  static constexpr size_t kRing = (size_t)kStages * kStage;
-  static constexpr uint32_t kPad = 32 * 128;  // bytes per warp: 128 bytes of each of 32 output rows
-  static constexpr size_t kSmem = kRing + kEpiWarps * kPad + 1024;
-  static constexpr int kCpt = TN / 2;
-  static constexpr int kGroups = TN / 8;  // groups of 8 columns, the unit of the exchange
-  static_assert(kStages % kBufs == 0, "stages and buffers share one unrolled loop");
-  static_assert((size_t)(kGroups + kMaxSplit) * 8 * kF8Block * 4 <= kRing, "the exchange reuses the ring");
-};
-
-// Stores chunks of 128 bytes per row (32 f32 or 64 bf16 columns) for the 32 rows a warp's lanes hold.
-// Through shared memory (16-byte pieces permuted by row, so neither side has bank conflicts): a
-// lane's own row would make every store touch 32 lines; this way one store instruction covers
-// whole lines of four rows.
+// Stores chunks of 32 bytes per row (8 f32 or 16 bf16 columns) for the 32 rows a warp's lanes hold.
+// Through shared memory (the two 16-byte pieces swapped in every other group of four rows, so that
+// neither side has bank conflicts): a lane's own row would make every store touch half a sector
+// of 32 lines; this way a store instruction covers whole sectors of 16 rows.
 struct RowStore {
+  static constexpr uint32_t kPad = 32 * 32;  // bytes of shared memory per warp
   const F8GemmParams& p;
-  uint32_t pad;   // this warp's 4 KB of shared memory
+  uint32_t pad;
   int lane;
   int64_t r0;     // the row of lane 0
   bool aligned;   // rows start on 16 bytes
 
-  // Piece j of this lane's row: 4 f32 or 8 bf16 values of columns n0 + j * 4 (8).
+  static __device__ __forceinline__ uint32_t place(int row, int j) { return row * 32 + ((j ^ ((row >> 2) & 1)) << 4); }
+  // Piece j of this lane's row: 4 f32 or 8 bf16 values.
   __device__ __forceinline__ void piece(int j, uint32_t a, uint32_t b, uint32_t c, uint32_t d) const {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(pad + lane * 128 + ((j ^ (lane & 7)) << 4)), "r"(a),
-                 "r"(b), "r"(c), "r"(d)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(pad + place(lane, j)), "r"(a), "r"(b), "r"(c), "r"(d)
                  : "memory");
   }
-  __device__ __forceinline__ uint4 at(int row, int j) const {
-    uint4 v;
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "r"(pad + row * 128 + ((j ^ (row & 7)) << 4))
-                 : "memory");
-    return v;
-  }
-  // The chunk that starts at column n0, `bytes` (at most 128, for the last columns less) of it.
+  // The chunk that starts at column n0 (those of its columns that exist).
   template <class T>
   __device__ __forceinline__ void out(int n0) const {
-    constexpr int kPer = 16 / sizeof(T);
+    constexpr int kPer = 16 / sizeof(T), kCols = 32 / sizeof(T);
     __syncwarp();
-    const int cols = min(128 / (int)sizeof(T), p.m.n - n0);
+    const int cols = min(kCols, p.m.n - n0);
     T* base = static_cast<T*>(p.out) + r0 * p.out_stride + n0;
-    if (aligned && cols == 128 / (int)sizeof(T)) {
-      const int j = lane & 7;
+    if (aligned && cols == kCols) {
+      const int j = lane & 1;
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const int row = i * 4 + (lane >> 3);
-        const uint4 v = at(row, j);
+      for (int i = 0; i < 2; i++) {
+        const int row = i * 16 + (lane >> 1);
+        uint4 v;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                     : "r"(pad + place(row, j))
+                     : "memory");
         if (r0 + row < p.rows) *reinterpret_cast<uint4*>(base + row * p.out_stride + j * kPer) = v;
       }
     } else {
       const int rows = (int)min((int64_t)32, p.rows - r0);
-      for (int row = 0; row < rows; row++)
-        for (int c = lane; c < cols; c += 32) {
-          const uint32_t from = pad + row * 128 + (((c / kPer) ^ (row & 7)) << 4) + c % kPer * sizeof(T);
-          if constexpr (sizeof(T) == 4) {
-            uint32_t v;
-            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(from) : "memory");
-            reinterpret_cast<uint32_t*>(base)[row * p.out_stride + c] = v;
-          } else {
-            uint16_t v;
-            asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(from) : "memory");
-            reinterpret_cast<uint16_t*>(base)[row * p.out_stride + c] = v;
-          }
+      for (int i = lane; i < rows * kCols; i += 32) {
+        const int row = i / kCols, c = i % kCols;
+        if (c >= cols) continue;
+        const uint32_t from = pad + place(row, c / kPer) + c % kPer * sizeof(T);
+        if constexpr (sizeof(T) == 4) {
+          uint32_t v;
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(from) : "memory");
+          reinterpret_cast<uint32_t*>(base)[row * p.out_stride + c] = v;
+        } else {
+          uint16_t v;
+          asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(from) : "memory");
+          reinterpret_cast<uint16_t*>(base)[row * p.out_stride + c] = v;
         }
+      }
     }
     __syncwarp();
   }
@@ -408,22 +387,76 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <int TN>
-__global__ void __launch_bounds__(Wide<TN>::kThreads, 1) f8_wide_kernel(const __grid_constant__ CUtensorMap tm_x,
-                                                                        const __grid_constant__ F8Args a) {
-  using C = Wide<TN>;
+// A thread's sums of columns [n0, n0 + N) of its row, plus the bias, stored by its warp.
+template <int N>
+__device__ __forceinline__ void store_sums(const RowStore& rs, uint64_t (&acc)[N / 2], int n0, bool bf16) {
+  const F8GemmParams& p = rs.p;
+  if (p.m.bias) {
+#pragma unroll
+    for (int c = 0; c < N; c += 2)
+      acc[c / 2] = pair_of(pair_lo(acc[c / 2]) + (n0 + c < p.m.n ? p.m.bias[n0 + c] : 0.f),
+                           pair_hi(acc[c / 2]) + (n0 + c + 1 < p.m.n ? p.m.bias[n0 + c + 1] : 0.f));
+  }
+  if (bf16) {
+#pragma unroll
+    for (int c = 0; c < N; c += 16) {
+      if (n0 + c >= p.m.n) break;
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const uint64_t* v = acc + c / 2 + 4 * j;
+        rs.piece(j, bf16_pair(pair_lo(v[0]), pair_hi(v[0])), bf16_pair(pair_lo(v[1]), pair_hi(v[1])),
+                 bf16_pair(pair_lo(v[2]), pair_hi(v[2])), bf16_pair(pair_lo(v[3]), pair_hi(v[3])));
+      }
+      rs.out<__nv_bfloat16>(n0 + c);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; c += 8) {
+      if (n0 + c >= p.m.n) break;
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const uint64_t* v = acc + c / 2 + 2 * j;
+        rs.piece(j, (uint32_t)v[0], (uint32_t)(v[0] >> 32), (uint32_t)v[1], (uint32_t)(v[1] >> 32));
+      }
+      rs.out<float>(n0 + c);
+    }
+  }
+}
+
+// ---- many rows: the rows are the MMA's M, C::kTN matrix rows its N --------------------------------
+
+// Bound by the tensor cores and by the operands' way from L2. With the rows as M, a thread of the
+// epilogue holds one row, so a block's scale is one number per thread (no shared-memory reads).
+// Persistent: a CTA takes every gridDim-th tile, and loads and products of the next tile run
+// while one is stored.
+struct Wide {
+  static constexpr int kTN = 128;
+  static constexpr int kEpiWarps = 8;
+  static constexpr int kThreads = (kEpiWarps + 2) * 32;  // + loader, MMA issuer
+  static constexpr uint32_t kStage = 2 * kTile;
+  static constexpr int kStages = 6;
+  static constexpr int kBufs = 4;
+  static constexpr size_t kRing = (size_t)kStages * kStage;
+  static constexpr size_t kSmem = kRing + kEpiWarps * RowStore::kPad + 1024;
+  static constexpr int kCpt = kTN / 2;
+  static constexpr int kGroups = kTN / 8;  // groups of 8 columns, the unit of the exchange
+  static_assert((size_t)(kGroups + kMaxSplit) * 8 * kF8Block * 4 <= kRing, "the exchange reuses the ring");
+};
+
+__global__ void __launch_bounds__(Wide::kThreads, 1) f8_wide_kernel(const __grid_constant__ CUtensorMap tm_x,
+                                                                    const __grid_constant__ F8Args a) {
+  using C = Wide;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages], tfull[C::kBufs], tempty[C::kBufs], gone;
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
   const F8GemmParams& p = a.p;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int S = a.split;
   const int rank = S > 1 ? (int)cluster_rank() : 0;
   const int first = blockIdx.x / S, stride = gridDim.x / S, total = a.ntiles * a.rtiles;
   const int b0 = (int)((int64_t)rank * a.kblocks / S), nb = (int)((int64_t)(rank + 1) * a.kblocks / S) - b0;
-  constexpr int kTiles = TN / kF8Block;  // packed tiles per stage
 
   if (tid == 0) {
     for (int i = 0; i < C::kStages; i++) {
@@ -446,25 +479,25 @@ __global__ void __launch_bounds__(Wide<TN>::kThreads, 1) f8_wide_kernel(const __
   pdl_wait();
 
   if (warp >= C::kEpiWarps) {
-    if (C::kShift) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == C::kEpiWarps && lane == 0) {
+    const bool lead = elect_one();
+    if (warp == C::kEpiWarps) {
       int issued = 0, st = 0;
       uint32_t parity = 1;
       bool ok = true;
       for (int tile = first; tile < total && ok; tile += stride) {
         const int nt = tile % a.ntiles, row = tile / a.ntiles * kF8Block;
-        const int have = min(kTiles, p.m.tiles() - nt * kTiles);
-        const uint8_t* w = p.m.w + ((int64_t)nt * kTiles * a.kblocks + b0) * kF8TileBytes;
-        const int64_t next = (int64_t)a.kblocks * kF8TileBytes;  // the same block of the next 128 matrix rows
+        const uint8_t* w = p.m.w + ((int64_t)nt * a.kblocks + b0) * kF8TileBytes;
         for (int b = b0; b < b0 + nb; b++, issued++, w += kF8TileBytes) {
           ok = role_wait(smem_addr(&empty[st]), parity, &failed);
           if (!ok) break;
-          uint64_t* bar = &full[st];
-          uint8_t* at = smem + (size_t)st * C::kStage;
-          mbar_expect_tx(bar, kTile * (1 + have));
-          tma_load_2d(at, &tm_x, b * kF8Block, row, bar);
-          bulk_g2s(at + kTile, w, kTile, bar);
-          if (kTiles > 1 && have > 1) bulk_g2s(at + 2 * kTile, w + next, kTile, bar);
+          if (lead) {
+            uint64_t* bar = &full[st];
+            uint8_t* at = smem + (size_t)st * C::kStage;
+            mbar_expect_tx(bar, C::kStage);
+            tma_load_2d(at, &tm_x, b * kF8Block, row, bar);
+            bulk_g2s(at + kTile, w, kTile, bar);
+          }
+          __syncwarp();
           if (++st == C::kStages) {
             st = 0;
             parity ^= 1;
@@ -473,31 +506,43 @@ __global__ void __launch_bounds__(Wide<TN>::kThreads, 1) f8_wide_kernel(const __
       }
       pdl_launch();
       drain_loads(full, issued, C::kStages);
-    } else if (warp == C::kEpiWarps + 1 && lane == 0) {
+    } else if (warp == C::kEpiWarps + 1) {
       // Tiles make no difference here: every block is a product of its own.
-      constexpr uint32_t idesc = idesc_e4m3(kF8Block, TN);
-      constexpr int kTurns = C::kStages / C::kBufs;  // of the buffers per pass over the stages
+      constexpr uint32_t idesc = idesc_e4m3(kF8Block, C::kTN);
       const uint32_t full_at = smem_addr(full), tempty_at = smem_addr(tempty);
       const uint64_t x_desc = sw128_desc(smem_addr(smem)), w_desc = sw128_desc(smem_addr(smem) + kTile);
-      uint32_t pass = 0;
-      bool ok = true;
-      for (int left = (total - first + stride - 1) / stride * nb; left > 0 && ok; left -= C::kStages, pass++) {
-#pragma unroll
-        for (int st = 0; st < C::kStages; st++) {
-          if (st >= left || !ok) break;
-          constexpr int kB = C::kBufs;
-          ok = role_wait(tempty_at + 8 * (st % kB), (pass * kTurns + st / kB + 1) & 1, &failed) &&
-               role_wait(full_at + 8 * st, pass & 1, &failed);
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int k = 0; k < 4; k++)
-            umma_f8(tmem + st % kB * TN, x_desc + (st * C::kStage >> 4) + 2 * k, w_desc + (st * C::kStage >> 4) + 2 * k, idesc, k != 0);
-          umma_commit(&empty[st]);
-          umma_commit(&tfull[st % kB]);
+      const int blocks = (total - first + stride - 1) / stride * nb;
+      int st = 0, buf = 0;
+      uint32_t parity = 0, turn = 1;
+      bool ok = true, free = true, here = mbar_test_at(full_at, 0);
+#pragma unroll 1
+      for (int i = 0; i < blocks; i++) {
+        ok = (free || role_wait(tempty_at + 8 * buf, turn, &failed)) && (here || role_wait(full_at + 8 * st, parity, &failed));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d = tmem + buf * C::kTN;
+        const uint64_t at = (uint64_t)(st * (C::kStage >> 4));
+        uint64_t *empty_bar = &empty[st], *tfull_bar = &tfull[buf];
+        if (++st == C::kStages) {
+          st = 0;
+          parity ^= 1;
         }
+        if (++buf == C::kBufs) {
+          buf = 0;
+          turn ^= 1;
+        }
+        // The next block's barriers are looked at while this block's products are issued.
+        free = mbar_test_at(tempty_at + 8 * buf, turn);
+        here = mbar_test_at(full_at + 8 * st, parity);
+        if (lead) {
+#pragma unroll
+          for (int k = 0; k < 4; k++) umma_f8(d, x_desc + at + 2 * k, w_desc + at + 2 * k, idesc, k != 0);
+          umma_commit(empty_bar);
+          umma_commit(tfull_bar);
+        }
+        __syncwarp();
       }
-      if (!ok) drain_mma(&gone);
+      if (!ok) drain_mma(&gone, lead);
     }
     if (S > 1) {
       __syncwarp();
@@ -505,11 +550,10 @@ __global__ void __launch_bounds__(Wide<TN>::kThreads, 1) f8_wide_kernel(const __
       cluster_sync();
     }
   } else {
-    if (C::kShift) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int half = warp >> 2, row_l = (warp & 3) * 32 + lane;
     const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * C::kCpt;
     const bool bf16 = p.out_bf16;
-    RowStore rs{p, smem_addr(smem + C::kRing) + warp * C::kPad, lane, 0,
+    RowStore rs{p, smem_addr(smem + C::kRing) + warp * RowStore::kPad, lane, 0,
                 reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.out_stride % (bf16 ? 8 : 4) == 0};
     auto bias_at = [&](int n) { return p.m.bias && n < p.m.n ? p.m.bias[n] : 0.f; };
     int buf = 0;
@@ -518,10 +562,9 @@ __global__ void __launch_bounds__(Wide<TN>::kThreads, 1) f8_wide_kernel(const __
       const int nt = tile % a.ntiles, rt = tile / a.ntiles;
       const int64_t r = (int64_t)rt * kF8Block + row_l;
       rs.r0 = r - lane;
-      const int wt = nt * kTiles + (kTiles > 1 ? half : 0);
-      const bool live = r < p.rows && wt < p.m.tiles();
+      const bool live = r < p.rows;
       const float* xs = p.scales + (int64_t)b0 * p.scale_stride + (live ? r : 0);
-      const float* ws = p.m.scales + (int64_t)(live ? wt : 0) * a.kblocks + b0;
+      const float* ws = p.m.scales + (int64_t)nt * a.kblocks + b0;
       uint64_t acc[C::kCpt / 2];
 #pragma unroll
       for (int i = 0; i < C::kCpt / 2; i++) acc[i] = 0;
@@ -548,15 +591,15 @@ __global__ void __launch_bounds__(Wide<TN>::kThreads, 1) f8_wide_kernel(const __
           const uint64_t sc2 = pair_of(sc, sc);
           fetch(j, b1 + j + 4);
 #pragma unroll
-          for (int c = 0; c < C::kCpt; c += 16) {
-            uint64_t t[8];
-            tmem_ld_pairs<16>(trow + buf * TN + c, t);
+          for (int c = 0; c < C::kCpt; c += 32) {
+            uint64_t t[16];
+            tmem_ld_pairs<32>(trow + buf * C::kTN + c, t);
 #pragma unroll
-            for (int e = 0; e < 8; e++) fma_pair(acc[c / 2 + e], t[e], sc2);
+            for (int e = 0; e < 16; e++) fma_pair(acc[c / 2 + e], t[e], sc2);
           }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&tempty[buf]);
+          if (lane == 0) mbar_arrive_relaxed(smem_addr(&tempty[buf]));
           if (++buf == C::kBufs) {
             buf = 0;
             parity ^= 1;
@@ -565,36 +608,7 @@ __global__ void __launch_bounds__(Wide<TN>::kThreads, 1) f8_wide_kernel(const __
       }
       if (S == 1) {
         if (!ok) break;
-        const int n0 = nt * TN + half * C::kCpt;
-        if (p.m.bias) {
-#pragma unroll
-          for (int c = 0; c < C::kCpt; c += 2)
-            acc[c / 2] = pair_of(pair_lo(acc[c / 2]) + bias_at(n0 + c), pair_hi(acc[c / 2]) + bias_at(n0 + c + 1));
-        }
-        if (bf16) {
-#pragma unroll
-          for (int c = 0; c < C::kCpt; c += 64) {
-            if (n0 + c >= p.m.n) break;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-              const uint64_t* v = acc + c / 2 + 4 * j;
-              rs.piece(j, bf16_pair(pair_lo(v[0]), pair_hi(v[0])), bf16_pair(pair_lo(v[1]), pair_hi(v[1])),
-                       bf16_pair(pair_lo(v[2]), pair_hi(v[2])), bf16_pair(pair_lo(v[3]), pair_hi(v[3])));
-            }
-            rs.out<__nv_bfloat16>(n0 + c);
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < C::kCpt; c += 32) {
-            if (n0 + c >= p.m.n) break;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-              const uint64_t* v = acc + c / 2 + 2 * j;
-              rs.piece(j, (uint32_t)v[0], (uint32_t)(v[0] >> 32), (uint32_t)v[1], (uint32_t)(v[1] >> 32));
-            }
-            rs.out<float>(n0 + c);
-          }
-        }
+        store_sums<C::kCpt>(rs, acc, nt * C::kTN + half * C::kCpt, bf16);
       } else {
         // One tile per cluster: its CTAs exchange their sums through the rings they are done
         // with, [rank][group of the owner][two float4][row]. Group g belongs to the rank whose
@@ -617,7 +631,7 @@ __global__ void __launch_bounds__(Wide<TN>::kThreads, 1) f8_wide_kernel(const __
         cluster_sync();
         const int g0 = rank * G / S, g1 = (rank + 1) * G / S;
         for (int g = g0 + half; g < g1; g += 2) {
-          const int n = nt * TN + g * 8;
+          const int n = nt * C::kTN + g * 8;
           if (n >= p.m.n) break;
           float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -662,6 +676,212 @@ __global__ void __launch_bounds__(Wide<TN>::kThreads, 1) f8_wide_kernel(const __
   if (warp == C::kEpiWarps + 1) tmem_free(tmem, 512);
 }
 
+// ---- very many rows: 128 x 256 tiles ---------------------------------------------------------------
+
+// The same with 256 matrix rows per tile (48 KB of operands per block for the work that takes 64 KB
+// as two tiles of 128: with the narrower tiles the operands' way from L2 is the bound). Scaling and
+// adding a block's 128 x 256 products takes the SM's FMA pipes 256 clocks of the 512 that the
+// products take, so it is spread over 16 warps, four per scheduler, each with 64 columns of 32
+// rows. A warp of its own fetches the rows' scales into shared memory, 8 blocks at a time.
+// Persistent: a CTA takes every gridDim-th tile, and loads and products of the next tile start
+// while one is stored.
+struct Big {
+  static constexpr int kTN = 256;
+  static constexpr int kEpiWarps = 16;
+  static constexpr int kThreads = (kEpiWarps + 4) * 32;  // + loader, MMA issuer, scales, one idle
+  static constexpr uint32_t kStage = 3 * kTile;
+  static constexpr int kStages = 4;
+  static constexpr int kBufs = 2;
+  static constexpr int kChunk = 8;  // blocks whose row scales are fetched at once
+  static constexpr size_t kRing = (size_t)kStages * kStage;
+  static constexpr size_t kSmem = kRing + kEpiWarps * RowStore::kPad + 2 * kChunk * kF8Block * 4 + 1024;
+  static constexpr int kCpt = kTN / 4;
+};
+
+__global__ void __launch_bounds__(Big::kThreads, 1) f8_big_kernel(const __grid_constant__ CUtensorMap tm_x,
+                                                                    const __grid_constant__ F8Args a) {
+  using C = Big;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* scale_ring = reinterpret_cast<float*>(smem + C::kRing + C::kEpiWarps * RowStore::kPad);  // [2][chunk][128 rows]
+  __shared__ __align__(8) uint64_t full[C::kStages], empty[C::kStages], tfull[C::kBufs], tempty[C::kBufs],
+      scaled[2], read[2], gone;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed;
+  const F8GemmParams& p = a.p;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const int first = blockIdx.x, stride = gridDim.x, total = a.ntiles * a.rtiles, nb = a.kblocks;
+
+  if (tid == 0) {
+    for (int i = 0; i < C::kStages; i++) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < C::kBufs; i++) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], C::kEpiWarps);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&scaled[i], 1);
+      mbar_init(&read[i], C::kEpiWarps);
+    }
+    mbar_init(&gone, 1);
+    failed = 0;
+    fence_mbar_init();
+  }
+  if (warp == C::kEpiWarps + 1) tmem_alloc(&tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  pdl_wait();
+
+  if (warp == C::kEpiWarps) {
+    const bool lead = elect_one();
+    int issued = 0, st = 0;
+    uint32_t parity = 1;
+    bool ok = true;
+    const int64_t next = (int64_t)nb * kF8TileBytes;  // the same block of the next 128 matrix rows
+    for (int tile = first; tile < total && ok; tile += stride) {
+      const int wt = tile % a.ntiles * 2, row = tile / a.ntiles * kF8Block;
+      const bool both = wt + 1 < p.m.tiles();
+      const uint8_t* w = p.m.w + (int64_t)wt * nb * kF8TileBytes;
+      for (int b = 0; b < nb; b++, issued++, w += kF8TileBytes) {
+        ok = role_wait(smem_addr(&empty[st]), parity, &failed);
+        if (!ok) break;
+        if (lead) {
+          uint64_t* bar = &full[st];
+          uint8_t* at = smem + (size_t)st * C::kStage;
+          mbar_expect_tx(bar, both ? 3 * kTile : 2 * kTile);
+          tma_load_2d(at, &tm_x, b * kF8Block, row, bar);
+          bulk_g2s(at + kTile, w, kTile, bar);
+          if (both) bulk_g2s(at + 2 * kTile, w + next, kTile, bar);
+        }
+        __syncwarp();
+        if (++st == C::kStages) {
+          st = 0;
+          parity ^= 1;
+        }
+      }
+    }
+    pdl_launch();
+    drain_loads(full, issued, C::kStages);
+  } else if (warp == C::kEpiWarps + 1) {
+    constexpr uint32_t idesc = idesc_e4m3(kF8Block, C::kTN);
+    const bool lead = elect_one();
+    const uint32_t full_at = smem_addr(full), tempty_at = smem_addr(tempty);
+    const uint64_t x_desc = sw128_desc(smem_addr(smem)), w_desc = sw128_desc(smem_addr(smem) + kTile);
+    const int blocks = (total - first + stride - 1) / stride * nb;
+    int st = 0, buf = 0;
+    uint32_t parity = 0, turn = 1;
+    bool ok = true;
+#pragma unroll 1
+    for (int i = 0; i < blocks; i++) {
+      ok = role_wait(full_at + 8 * st, parity, &failed) && role_wait(tempty_at + 8 * buf, turn, &failed);
+      if (!ok) break;
+      tc_fence_after();
+      if (lead) {
+        const uint64_t at = (uint64_t)(st * (C::kStage >> 4));
+#pragma unroll
+        for (int k = 0; k < 4; k++) umma_f8(tmem + buf * C::kTN, x_desc + at + 2 * k, w_desc + at + 2 * k, idesc, k != 0);
+        umma_commit(&tfull[buf]);
+        umma_commit(&empty[st]);
+      }
+      __syncwarp();
+      if (++st == C::kStages) {
+        st = 0;
+        parity ^= 1;
+      }
+      buf ^= 1;
+      turn ^= buf == 0;
+    }
+    if (!ok) drain_mma(&gone, lead);
+  } else if (warp == C::kEpiWarps + 2) {
+    int slot = 0;
+    uint32_t parity = 1;
+    bool ok = true;
+    for (int tile = first; tile < total && ok; tile += stride) {
+      const int64_t r0 = (int64_t)(tile / a.ntiles) * kF8Block + lane * 4;
+      for (int i0 = 0; i0 < nb; i0 += C::kChunk) {
+        float x[C::kChunk][4];
+#pragma unroll
+        for (int j = 0; j < C::kChunk; j++) {
+          const float* xs = p.scales + (int64_t)(i0 + j) * p.scale_stride + r0;
+#pragma unroll
+          for (int e = 0; e < 4; e++) x[j][e] = i0 + j < nb && r0 + e < p.rows ? xs[e] : 0.f;
+        }
+        ok = role_wait(smem_addr(&read[slot]), parity, &failed);
+        if (!ok) break;
+        float4* to = reinterpret_cast<float4*>(scale_ring + slot * C::kChunk * kF8Block) + lane;
+#pragma unroll
+        for (int j = 0; j < C::kChunk; j++) to[j * 32] = make_float4(x[j][0], x[j][1], x[j][2], x[j][3]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&scaled[slot]);
+        slot ^= 1;
+        parity ^= slot == 0;
+      }
+    }
+  } else if (warp < C::kEpiWarps) {
+    const int cg = warp >> 2, row_l = (warp & 3) * 32 + lane;
+    const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16) + cg * C::kCpt;
+    int buf = 0, slot = 0;
+    uint32_t parity = 0, turn = 0;
+    bool ok = true;
+    for (int tile = first; tile < total && ok; tile += stride) {
+      const int n0 = tile % a.ntiles * C::kTN + cg * C::kCpt;
+      const float* ws = p.m.scales + (int64_t)min(n0 / kF8Block, p.m.tiles() - 1) * nb;
+      uint64_t acc[C::kCpt / 2];
+#pragma unroll
+      for (int i = 0; i < C::kCpt / 2; i++) acc[i] = 0;
+      float sw = ws[0];
+#pragma unroll 1
+      for (int i0 = 0; i0 < nb && ok; i0 += C::kChunk) {
+        ok = role_wait(smem_addr(&scaled[slot]), turn, &failed);
+        if (!ok) break;
+        const float* xs = scale_ring + slot * C::kChunk * kF8Block + row_l;
+        const int end = min(nb, i0 + C::kChunk);
+#pragma unroll 1
+        for (int b = i0; b < end; b++, xs += kF8Block) {
+          const float sc = *xs * sw;
+          const uint64_t sc2 = pair_of(sc, sc);
+          sw = ws[min(b + 1, nb - 1)];
+          ok = role_wait(smem_addr(&tfull[buf]), parity, &failed);
+          if (!ok) break;
+          __syncwarp();
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < C::kCpt; c += 16) {
+            uint64_t t[8];
+            tmem_ld_pairs<16>(trow + buf * C::kTN + c, t);
+#pragma unroll
+            for (int e = 0; e < 8; e++) fma_pair(acc[c / 2 + e], t[e], sc2);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_relaxed(smem_addr(&tempty[buf]));
+          buf ^= 1;
+          parity ^= buf == 0;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&read[slot]);
+        slot ^= 1;
+        turn ^= slot == 0;
+      }
+      if (!ok) break;
+      const bool bf16 = p.out_bf16;
+      const RowStore rs{p, smem_addr(smem + C::kRing) + warp * RowStore::kPad, lane,
+                        (int64_t)(tile / a.ntiles) * kF8Block + (warp & 3) * 32,
+                        reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.out_stride % (bf16 ? 8 : 4) == 0};
+      store_sums<C::kCpt>(rs, acc, n0, bf16);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && failed && p.err) atomicExch(p.err, 2);
+  if (warp == C::kEpiWarps + 1) tmem_free(tmem, 512);
+}
+
 // ---- host side ----------------------------------------------------------------------------
 
 bool make_rows_map(CUtensorMap* map, const uint8_t* base, int64_t rows, int k, int64_t stride, int box_rows) {
@@ -697,55 +917,75 @@ void launch(dim3 grid, int threads, size_t smem, int split, const CUtensorMap& m
   check_cuda(cudaLaunchKernelEx(&cfg, kernel, map, a), "product launch");
 }
 
-// CTAs per cluster so that `tiles` tiles fill `slots` CTAs, each with at least `least` blocks.
-int choose_split(int64_t tiles, int kblocks, int slots, int least) {
-  const int64_t s = std::min<int64_t>({slots / std::max<int64_t>(tiles, 1), kMaxSplit, kblocks / least});
-  return (int)std::max<int64_t>(s, 1);
+constexpr int kSms = 148;
+
+// The rows' map and the tiles of tn matrix rows x br rows.
+CUtensorMap plan(F8Args& a, int tn, int br) {
+  CUtensorMap map;
+  if (!make_rows_map(&map, a.p.q, a.p.rows, a.p.m.k, a.p.q_stride, br))
+    throw Error(SVL_ERR_CUDA, "cannot encode the rows' TMA tensor map");
+  a.ntiles = (a.p.m.n + tn - 1) / tn;
+  a.rtiles = (int)((a.p.rows + br - 1) / br);
+  if ((int64_t)a.ntiles * a.rtiles > INT32_MAX / kMaxSplit) throw Error(SVL_ERR_UNSUPPORTED, "too many output tiles");
+  return map;
 }
 
+// Up to 64 rows. Clusters of 4 (2) as long as 200 CTAs are not exceeded and each has two blocks: the
+// SMs that a few tiles leave idle then load too (1 x 2048 x 2048: 5.2 us alone, 4.0 with 2, 3.4 with
+// 4, 3.6 with 8; 1 x 11264 x 2048, 88 tiles: 5.9 alone, 6.2 with 2, 9.6 with 4). Clusters of 8 only
+// for very long axes (1 x 2560 x 10240: 8.4 us with 4, 7.2 with 8), other sizes never won.
 template <int BN>
 void launch_thin(F8Args a, cudaStream_t s) {
-  CUtensorMap map;
-  if (!make_rows_map(&map, a.p.q, a.p.rows, a.p.m.k, a.p.q_stride, BN))
-    throw Error(SVL_ERR_CUDA, "cannot encode the rows' TMA tensor map");
-  a.ntiles = a.p.m.tiles();
-  a.rtiles = (int)((a.p.rows + BN - 1) / BN);
-  a.split = choose_split((int64_t)a.ntiles * a.rtiles, a.kblocks, 2 * 148, 1);
+  const CUtensorMap map = plan(a, kF8Block, BN);
+  const int tiles = a.ntiles * a.rtiles;
+  a.split = 1;
+  while (a.split < 4 && tiles * a.split * 2 <= 200 && a.kblocks >= a.split * 4) a.split *= 2;
+  if (a.split == 4 && tiles * 8 <= 200 && a.kblocks >= 80) a.split = 8;
   launch<f8_thin_kernel<BN>>(dim3(a.ntiles * a.split, a.rtiles), Thin<BN>::kThreads, Thin<BN>::kSmem, a.split, map, a, s);
 }
 
-template <int TN>
+// 128 x 128 tiles. The exchange of a split tile costs about as much as 9 blocks, so it is split only
+// where it saves more (256 x 2048 x 5632, 32 tiles: 16.5 us alone, 12.5 with 2, 10.4 with 4; 256 x
+// 6144 x 2048, 96 tiles: 9.3 alone, 16.9 with 2), and where outputs can be stored in 16-byte pieces.
 void launch_wide(F8Args a, cudaStream_t s) {
-  CUtensorMap map;
-  if (!make_rows_map(&map, a.p.q, a.p.rows, a.p.m.k, a.p.q_stride, kF8Block))
-    throw Error(SVL_ERR_CUDA, "cannot encode the rows' TMA tensor map");
-  a.ntiles = (a.p.m.n + TN - 1) / TN;
-  a.rtiles = (int)((a.p.rows + kF8Block - 1) / kF8Block);
-  const int64_t tiles = (int64_t)a.ntiles * a.rtiles;
-  if (tiles > INT32_MAX) throw Error(SVL_ERR_UNSUPPORTED, "too many output tiles");
-  a.split = choose_split(tiles, a.kblocks, 148, 2);
-  const int grid = a.split > 1 ? (int)tiles * a.split : (int)std::min<int64_t>(tiles, 148);
-  launch<f8_wide_kernel<TN>>(dim3(grid), Wide<TN>::kThreads, Wide<TN>::kSmem, a.split, map, a, s);
+  const CUtensorMap map = plan(a, Wide::kTN, kF8Block);
+  const int tiles = a.ntiles * a.rtiles;
+  const bool aligned = reinterpret_cast<uintptr_t>(a.p.out) % 16 == 0 && a.p.out_stride % (a.p.out_bf16 ? 8 : 4) == 0;
+  a.split = 1;
+  if (aligned)
+    for (int S : {2, 4})
+      if (tiles * S <= kSms && a.kblocks * (S - 1) > 9 * S) a.split = S;
+  const int grid = a.split > 1 ? tiles * a.split : std::min(tiles, kSms);
+  launch<f8_wide_kernel>(dim3(grid), Wide::kThreads, Wide::kSmem, a.split, map, a, s);
+}
+
+void launch_big(F8Args a, cudaStream_t s) {
+  const CUtensorMap map = plan(a, Big::kTN, kF8Block);
+  a.split = 1;
+  launch<f8_big_kernel>(dim3(std::min(a.ntiles * a.rtiles, kSms)), Big::kThreads, Big::kSmem, 1, map, a, s);
 }
 
 }  // namespace
 
+// Which kernel. Up to 16 rows, 32, and 64 as long as two tiles of 32 rows per matrix tile fit the
+// SMs: the matrix rows as M (64 x 2048 x 2048: 5.1 us against 7.6 as a 128 x 128 tile; 64 x 11264 x
+// 2048, 176 tiles: 9.9 against 8.9). Above, 128 x 128 tiles or 128 x 256: a wave of the larger ones
+// takes 1.55 times as long (1024 x 11264 x 2048: 35 us in 5 waves, 33 in 3; 512 x 11264 x 2048: 22 us
+// in 3, 23 in 2; 256 x 11264 x 2048: 15.5 us in 2, 13.3 in 1).
 void launch_f8_gemm(const F8GemmParams& p, cudaStream_t s) {
   F8Args a{};
   a.p = p;
   a.kblocks = p.m.kblocks();
+  const int64_t rt = (p.rows + kF8Block - 1) / kF8Block;
+  const int64_t wide_waves = (rt * p.m.tiles() + kSms - 1) / kSms, big_waves = (rt * ((p.m.tiles() + 1) / 2) + kSms - 1) / kSms;
   if (p.rows <= 16)
     launch_thin<16>(a, s);
-  else if (p.rows <= 32)
+  else if (p.rows <= 32 || (p.rows <= 64 && 2 * p.m.tiles() <= kSms))
     launch_thin<32>(a, s);
-  else if (p.rows <= 64)
-    launch_thin<64>(a, s);
-  else if (p.rows <= 128)
-    launch_thin<128>(a, s);
-  else if ((p.rows + 127) / 128 * ((p.m.n + 255) / 256) < 148)
-    launch_wide<128>(a, s);
+  else if (big_waves * 31 < wide_waves * 20)
+    launch_big(a, s);
   else
-    launch_wide<256>(a, s);
+    launch_wide(a, s);
 }
 
 }  // namespace svl

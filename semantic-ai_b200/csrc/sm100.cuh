@@ -47,6 +47,24 @@ __device__ __forceinline__ bool mbar_try_wait_at(uint32_t bar, uint32_t parity) 
       : "memory");
   return ok != 0;
 }
+// Whether the phase is over, without waiting.
+__device__ __forceinline__ bool mbar_test_at(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Arrivals that order nothing but the arrival itself: for tensor-memory buffers, whose reads the
+// arriving thread has waited for and fenced (tcgen05.wait::ld, tcgen05.fence::before_thread_sync). A
+// release would also wait for the thread's global loads in flight, hundreds of clocks.
+__device__ __forceinline__ void mbar_arrive_relaxed(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 // Bounded wait on a phase of an mbarrier; false when it ran out.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint32_t limit = kWaitLimit) {
   for (uint32_t i = 0; i < limit; i++)
@@ -97,6 +115,16 @@ __device__ __forceinline__ void prefetch_l2_share(const uint8_t* base, int64_t b
   const int64_t a = (int64_t)cta * share;
   const int64_t e = min(a + share, bytes / 16 * 16);
   for (int64_t o = a; o < e; o += 65536) prefetch_l2(base + o, (uint32_t)(e - o < 65536 ? e - o : 65536), pol);
+}
+// True in one lane of the warp (all of whose lanes call this), the same one every time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
 }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

@@ -189,7 +189,7 @@ def check_linear(got, d, out):
 @pytest.mark.parametrize("rows,n,k", [
     (1, 1, 1), (1, 8, 16), (2, 100, 130), (1, 2048, 2048), (1, 8000, 2048), (15, 4001, 1000), (16, 256, 5632), (17, 129, 128), (31, 384, 640),
     (33, 1000, 2560), (64, 6144, 2048), (65, 512, 2047), (127, 130, 257), (128, 128, 128), (129, 2048, 5632), (255, 4001, 333),
-    (256, 11264, 2048), (257, 640, 1024), (515, 4001, 2500), (1000, 2048, 10240), (2049, 1111, 999)])
+    (256, 11264, 2048), (257, 640, 1024), (515, 4001, 2500), (1000, 2048, 10240), (2049, 1111, 999), (1500, 4001, 700), (8191, 2300, 300), (4000, 2560, 2048)])
 def test_linear(svl_lib, rows, n, k, out):
     import svl
     d = quantised(rows, k, n, rows + n + k, bias=(rows + n) % 2 == 0)
