@@ -23,41 +23,59 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// Eight consecutive values of a row of the stream as f32; `have` of them exist.
-template <class T>
-__device__ __forceinline__ void load8(const T* p, int have, bool wide, float (&v)[8]) {
-  if (wide && have == 8) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-      const uint4 a = *reinterpret_cast<const uint4*>(p);
-      v[0] = bf16_lo(a.x); v[1] = bf16_hi(a.x); v[2] = bf16_lo(a.y); v[3] = bf16_hi(a.y);
-      v[4] = bf16_lo(a.z); v[5] = bf16_hi(a.z); v[6] = bf16_lo(a.w); v[7] = bf16_hi(a.w);
-    }
-  } else {
+// V consecutive values of a row as they lie in memory; `have` of them exist. `wide`: the row starts
+// on 16 bytes.
+template <class T, int V>
+struct Raw {
+  uint4 v[V * sizeof(T) / 16];
+};
+template <class T, int V>
+__device__ __forceinline__ Raw<T, V> load_raw(const T* p, int have, bool wide) {
+  Raw<T, V> r;
+  if (wide && have >= V) {
 #pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = j < have ? (float)p[j] : 0.f;
+    for (int i = 0; i < (int)(V * sizeof(T) / 16); i++) r.v[i] = reinterpret_cast<const uint4*>(p)[i];
+  } else {
+    T* e = reinterpret_cast<T*>(r.v);
+#pragma unroll
+    for (int j = 0; j < V; j++) e[j] = j < have ? p[j] : T(0.f);
+  }
+  return r;
+}
+template <class T, int V>
+__device__ __forceinline__ void store_raw(T* p, const Raw<T, V>& r, int have, bool wide) {
+  if (wide && have >= V) {
+#pragma unroll
+    for (int i = 0; i < (int)(V * sizeof(T) / 16); i++) reinterpret_cast<uint4*>(p)[i] = r.v[i];
+  } else {
+    const T* e = reinterpret_cast<const T*>(r.v);
+#pragma unroll
+    for (int j = 0; j < V; j++)
+      if (j < have) p[j] = e[j];
   }
 }
-template <class T>
-__device__ __forceinline__ void store8(T* p, int have, bool wide, const float (&v)[8]) {
-  if (wide && have == 8) {
-    if constexpr (sizeof(T) == 4) {
-      reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      __nv_bfloat162 h[4];
+template <class T, int V>
+__device__ __forceinline__ void unpack(const Raw<T, V>& r, float (&v)[V]) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(r.v);
 #pragma unroll
-      for (int j = 0; j < 4; j++) h[j] = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-      *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(h);
-    }
+  for (int j = 0; j < V; j++) v[j] = sizeof(T) == 4 ? __uint_as_float(w[j]) : j & 1 ? bf16_hi(w[j / 2]) : bf16_lo(w[j / 2]);
+}
+// Rounded to the stream's type.
+template <class T, int V>
+__device__ __forceinline__ Raw<T, V> pack(const float (&v)[V]) {
+  Raw<T, V> r;
+  uint32_t* w = reinterpret_cast<uint32_t*>(r.v);
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < V; j++) w[j] = __float_as_uint(v[j]);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; j++)
-      if (j < have) p[j] = sizeof(T) == 4 ? (T)v[j] : (T)__float2bfloat16_rn(v[j]);
+    for (int j = 0; j < V; j += 2) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[j], v[j + 1]);
+      w[j / 2] = *reinterpret_cast<const uint32_t*>(&h);
+    }
   }
+  return r;
 }
 
 // The sum of v over a row's threads (a multiple of 32, threadIdx.x of them): warp sums, then the
@@ -73,111 +91,129 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
   return s;
 }
 
-// A row's threads (threadIdx.x) hold the whole row in registers, I pieces of 8 values each, so x
-// and the residual are read once: bound by HBM. 16 consecutive threads hold a block of 128
-// columns, whose maximum takes four shuffles. Short rows share a CTA (threadIdx.y).
-template <class T, int I>
-__global__ void __launch_bounds__(I == 4 ? 1024 : 512) norm_f8_kernel(const NormF8Params p) {
-  __shared__ float red_sm[2][32];
-  const int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+// A row's threads (threadIdx.x) hold the whole row in registers, I pieces of V values each (8 f32
+// or 16 bf16: 32 bytes), so x and the residual are read once: bound by HBM. 128 / V consecutive
+// threads hold a block of 128 columns. Short rows share a CTA (threadIdx.y). With many rows
+// a CTA goes through several of them and has the next one's x and residual on their way while it
+// works on one, since sums, scales and stores leave the memory idle otherwise.
+template <class T, int V, int I>
+__global__ void __launch_bounds__(I == 4 ? 1024 : 512) norm_f8_kernel(const __grid_constant__ NormF8Params p) {
+  __shared__ float red_sm[2][2][32];
+  const int64_t step = (int64_t)gridDim.x * blockDim.y;
+  int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   pdl_launch();
   pdl_wait();
   if (r >= p.rows) return;
-  // A CTA's rows use disjoint parts of red (blockDim.x / 32 * blockDim.y <= 32 warps).
-  float* red = red_sm[0] + threadIdx.y * (blockDim.x >> 5);
-  float* red2 = red_sm[1] + threadIdx.y * (blockDim.x >> 5);
-  const T* x = static_cast<const T*>(p.x) + r * p.x_stride;
-  const T* res = p.residual ? static_cast<const T*>(p.residual) + r * p.residual_stride : nullptr;
-  T* sum = p.sum ? static_cast<T*>(p.sum) + r * p.sum_stride : nullptr;
-  const bool xw = reinterpret_cast<uintptr_t>(x) % 16 == 0, rw = reinterpret_cast<uintptr_t>(res) % 16 == 0,
-             sw = reinterpret_cast<uintptr_t>(sum) % 16 == 0;
+  const int width = blockDim.x;
+  const bool xw = (reinterpret_cast<uintptr_t>(p.x) | (uint64_t)p.x_stride * sizeof(T)) % 16 == 0,
+             rw = (reinterpret_cast<uintptr_t>(p.residual) | (uint64_t)p.residual_stride * sizeof(T)) % 16 == 0,
+             sw = (reinterpret_cast<uintptr_t>(p.sum) | (uint64_t)p.sum_stride * sizeof(T)) % 16 == 0;
   const bool ww = reinterpret_cast<uintptr_t>(p.weight) % 16 == 0, bw = reinterpret_cast<uintptr_t>(p.bias) % 16 == 0;
-  float h[I][8];
-#pragma unroll
-  for (int i = 0; i < I; i++) {
-    const int c = (threadIdx.x + i * blockDim.x) * 8;
-    load8(x + c, min(8, p.k - c), xw, h[i]);
-  }
-  if (res) {
+  Raw<T, V> nx[I], nr[I];
+  auto fetch = [&](int64_t row) {
 #pragma unroll
     for (int i = 0; i < I; i++) {
-      const int c = (threadIdx.x + i * blockDim.x) * 8;
-      float a[8];
-      load8(res + c, min(8, p.k - c), rw, a);
-#pragma unroll
-      for (int j = 0; j < 8; j++) h[i][j] = sizeof(T) == 4 ? h[i][j] + a[j] : round_bf16(h[i][j] + a[j]);
+      const int c = (threadIdx.x + i * width) * V;
+      nx[i] = load_raw<T, V>(static_cast<const T*>(p.x) + row * p.x_stride + c, p.k - c, xw);
+      if (p.residual) nr[i] = load_raw<T, V>(static_cast<const T*>(p.residual) + row * p.residual_stride + c, p.k - c, rw);
     }
-  }
-  if (sum) {
+  };
+  constexpr bool kAhead = I < 4;  // the longest rows leave no registers for a second one
+  if (kAhead) fetch(r);
+  for (int turn = 0; r < p.rows; r += step, turn ^= 1) {
+    // A CTA's rows use disjoint parts of red (blockDim.x / 32 * blockDim.y <= 32 warps), and a row
+    // and the next one different halves.
+    float* red = red_sm[turn][0] + threadIdx.y * (width >> 5);
+    float* red2 = red_sm[turn][1] + threadIdx.y * (width >> 5);
+    float h[I][V];
+    if (!kAhead) fetch(r);
 #pragma unroll
     for (int i = 0; i < I; i++) {
-      const int c = (threadIdx.x + i * blockDim.x) * 8;
-      store8(sum + c, min(8, p.k - c), sw, h[i]);
+      unpack(nx[i], h[i]);
+      if (p.residual) {
+        float a[V];
+        unpack(nr[i], a);
+#pragma unroll
+        for (int j = 0; j < V; j++) h[i][j] = h[i][j] + a[j];
+        nx[i] = pack<T, V>(h[i]);
+        unpack(nx[i], h[i]);
+      }
+      if (p.sum) {
+        const int c = (threadIdx.x + i * width) * V;
+        store_raw(static_cast<T*>(p.sum) + r * p.sum_stride + c, nx[i], p.k - c, sw);
+      }
     }
-  }
-  if (p.norm != NORM_NONE) {
-    float a = 0.f;
-    if (p.norm == NORM_LAYER) {
+    if (kAhead && r + step < p.rows) fetch(r + step);
+    if (p.norm != NORM_NONE) {
+      float a = 0.f;
+      if (p.norm == NORM_LAYER) {
+#pragma unroll
+        for (int i = 0; i < I; i++)
+#pragma unroll
+          for (int j = 0; j < V; j++) a += h[i][j];
+        const float mean = row_sum(a, red2) / (float)p.k;
+#pragma unroll
+        for (int i = 0; i < I; i++) {
+          const int c = (threadIdx.x + i * width) * V;
+#pragma unroll
+          for (int j = 0; j < V; j++) h[i][j] = c + j < p.k ? h[i][j] - mean : 0.f;
+        }
+        a = 0.f;
+      }
 #pragma unroll
       for (int i = 0; i < I; i++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) a += h[i][j];
-      const float mean = row_sum(a, red2) / (float)p.k;
+        for (int j = 0; j < V; j++) a = fmaf(h[i][j], h[i][j], a);
+      const float rstd = 1.0f / sqrtf(row_sum(a, red) / (float)p.k + p.eps);
 #pragma unroll
       for (int i = 0; i < I; i++) {
-        const int c = (threadIdx.x + i * blockDim.x) * 8;
+        const int c = (threadIdx.x + i * width) * V, have = p.k - c;
 #pragma unroll
-        for (int j = 0; j < 8; j++) h[i][j] = c + j < p.k ? h[i][j] - mean : 0.f;
+        for (int j = 0; j < V; j++) h[i][j] = h[i][j] * rstd;
+        float a8[V];
+        if (p.weight) {
+          unpack(load_raw<float, V>(p.weight + c, have, ww), a8);
+#pragma unroll
+          for (int j = 0; j < V; j++) h[i][j] = h[i][j] * a8[j];
+        }
+        if (p.bias && p.norm == NORM_LAYER) {
+          unpack(load_raw<float, V>(p.bias + c, have, bw), a8);
+#pragma unroll
+          for (int j = 0; j < V; j++) h[i][j] = h[i][j] + a8[j];
+        }
       }
-      a = 0.f;
     }
-#pragma unroll
-    for (int i = 0; i < I; i++)
-#pragma unroll
-      for (int j = 0; j < 8; j++) a = fmaf(h[i][j], h[i][j], a);
-    const float rstd = 1.0f / sqrtf(row_sum(a, red) / (float)p.k + p.eps);
+    uint8_t* q = p.q + r * p.q_stride;
 #pragma unroll
     for (int i = 0; i < I; i++) {
-      const int c = (threadIdx.x + i * blockDim.x) * 8, have = min(8, p.k - c);
+      const int c = (threadIdx.x + i * width) * V, have = p.k - c;
+      // Values past the row's end are zero up to here (0 * rstd * 0 + 0).
+      float top = kF8Tiny;
 #pragma unroll
-      for (int j = 0; j < 8; j++) h[i][j] = h[i][j] * rstd;
-      float a8[8];
-      if (p.weight) {
-        load8(p.weight + c, have, ww, a8);
+      for (int j = 0; j < V; j++) top = max_nan(top, fabsf(h[i][j]));
 #pragma unroll
-        for (int j = 0; j < 8; j++) h[i][j] = h[i][j] * a8[j];
+      for (int o = kF8Block / V / 2; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float inv = __fdiv_rn(kF8Max, top);
+      if (have >= V) {
+        uint32_t e[V / 4];
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+          const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(h[i][j] * inv, h[i][j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+          const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(h[i][j + 2] * inv, h[i][j + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+          e[j / 4] = lo | hi << 16;
+        }
+        if constexpr (V == 16)
+          *reinterpret_cast<uint4*>(q + c) = make_uint4(e[0], e[1], e[2], e[3]);
+        else
+          *reinterpret_cast<uint2*>(q + c) = make_uint2(e[0], e[1]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; j++)
+          if (j < have) q[c + j] = to_e4m3(h[i][j] * inv);
       }
-      if (p.bias && p.norm == NORM_LAYER) {
-        load8(p.bias + c, have, bw, a8);
-#pragma unroll
-        for (int j = 0; j < 8; j++) h[i][j] = h[i][j] + a8[j];
-      }
+      if (threadIdx.x % (kF8Block / V) == 0 && have > 0)
+        p.scales[(int64_t)(c / kF8Block) * p.scale_stride + r] = __fdiv_rn(top, kF8Max);
     }
-  }
-  uint8_t* q = p.q + r * p.q_stride;
-#pragma unroll
-  for (int i = 0; i < I; i++) {
-    const int c = (threadIdx.x + i * blockDim.x) * 8, have = p.k - c;
-    float top = kF8Tiny;
-#pragma unroll
-    for (int j = 0; j < 8; j++) top = max_nan(top, j < have ? fabsf(h[i][j]) : 0.f);
-#pragma unroll
-    for (int o = 8; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float inv = __fdiv_rn(kF8Max, top);
-    if (have >= 8) {
-      uint2 v;
-      uint16_t* e = reinterpret_cast<uint16_t*>(&v);
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-        e[j] = __nv_cvt_float2_to_fp8x2(make_float2(h[i][2 * j] * inv, h[i][2 * j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-      *reinterpret_cast<uint2*>(q + c) = v;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; j++)
-        if (j < have) q[c + j] = to_e4m3(h[i][j] * inv);
-    }
-    if ((threadIdx.x & 15) == 0 && have > 0)
-      p.scales[(int64_t)(c / kF8Block) * p.scale_stride + r] = __fdiv_rn(top, kF8Max);
   }
 }
 
@@ -224,27 +260,78 @@ __global__ void __launch_bounds__(256) f8_quantise_kernel(const float* src, int 
 
 }  // namespace
 
-// Pieces per thread: one up to 4,096 columns (512 threads), then two and four, so that a CTA stays
-// small enough for several per SM; rows below 2,048 columns share CTAs of 256 threads.
-void launch_norm_f8(const NormF8Params& p, cudaStream_t s) {
-  const int pieces = (p.k + 7) / 8;
-  const int per = pieces <= 512 ? 1 : pieces <= 1024 ? 2 : 4;
-  const int threads = ((pieces + per - 1) / per + 31) / 32 * 32;
-  const int share = (int)std::min<int64_t>(std::max(1, 256 / threads), p.rows);
-  const int64_t grid = (p.rows + share - 1) / share;
-  if (grid > INT32_MAX) throw Error(SVL_ERR_UNSUPPORTED, "too many rows");
-  auto kernel = p.bf16 ? (per == 1 ? norm_f8_kernel<__nv_bfloat16, 1> : per == 2 ? norm_f8_kernel<__nv_bfloat16, 2> : norm_f8_kernel<__nv_bfloat16, 4>)
-                       : (per == 1 ? norm_f8_kernel<float, 1> : per == 2 ? norm_f8_kernel<float, 2> : norm_f8_kernel<float, 4>);
+namespace {
+
+// How a kernel's rows of `warps` warps share an SM best: rows per CTA and CTAs per SM. An SM gives
+// registers to four warps at a time, so that rows of five warps alone leave a third of it idle
+// (16384 x 2560 bf16: 4 rows of 5 warps at once 64 us, 6 in CTAs of
+// three 59 us). Asked of the runtime once per kernel and width.
+struct Shape {
+  int share, ctas;
+};
+template <class T, int V, int I>
+Shape shape_of(int warps) {
+  static std::atomic<uint32_t> known[33];
+  uint32_t v = known[warps].load(std::memory_order_relaxed);
+  if (!v) {
+    int best = 0;
+    for (int share = 1; share <= 8 && share * warps * 32 <= (I == 4 ? 1024 : 512); share++) {
+      int ctas = 0;
+      check_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, norm_f8_kernel<T, V, I>, share * warps * 32, 0), "occupancy");
+      if (share * ctas > best) {
+        best = share * ctas;
+        v = (uint32_t)share << 16 | (uint32_t)ctas;
+      }
+    }
+    if (!v) throw Error(SVL_ERR_CUDA, "the norm's kernel does not fit an SM");
+    known[warps].store(v, std::memory_order_relaxed);
+  }
+  return {(int)(v >> 16), (int)(v & 0xffff)};
+}
+
+template <class T, int V, int I>
+void launch_norm(const NormF8Params& p, cudaStream_t s) {
+  const int warps = ((p.k + V * I - 1) / (V * I) + 31) / 32;
+  Shape sh = shape_of<T, V, I>(warps);
+  // Few rows go to as many SMs as there are.
+  const int64_t spread = std::max<int64_t>(1, p.rows / 148);
+  if (sh.share > spread) sh.share = (int)spread;
+  const int64_t ctas = (p.rows + sh.share - 1) / sh.share;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(threads, share);
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>(ctas, 148 * sh.ctas));
+  cfg.blockDim = dim3(warps * 32, sh.share);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  check_cuda(cudaLaunchKernelEx(&cfg, kernel, p), "norm launch");
+  check_cuda(cudaLaunchKernelEx(&cfg, norm_f8_kernel<T, V, I>, p), "norm launch");
+}
+
+}  // namespace
+
+// 32 bytes of the stream per thread and piece, 16 of short bf16 rows (16384 x 256: 8 us against
+// 14) and of rows too long for 1,024 threads and two pieces.
+void launch_norm_f8(const NormF8Params& p, cudaStream_t s) {
+  using B = __nv_bfloat16;
+  if (p.bf16) {
+    if (p.k <= 512)
+      launch_norm<B, 8, 1>(p, s);
+    else if (p.k <= 8192)
+      launch_norm<B, 16, 1>(p, s);
+    else if (p.k <= 16384)
+      launch_norm<B, 16, 2>(p, s);
+    else
+      launch_norm<B, 8, 4>(p, s);
+  } else {
+    if (p.k <= 4096)
+      launch_norm<float, 8, 1>(p, s);
+    else if (p.k <= 8192)
+      launch_norm<float, 8, 2>(p, s);
+    else
+      launch_norm<float, 8, 4>(p, s);
+  }
 }
 
 void launch_f8_pack(const uint8_t* src, int64_t stride, int n, int k, uint8_t* dst, cudaStream_t s) {
