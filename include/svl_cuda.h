@@ -49,8 +49,17 @@ typedef enum { SVL_FFN_PLAIN_GELU_TANH = 0, SVL_FFN_PLAIN_GELU_ERF = 1, SVL_FFN_
 /* Norm (nn/transformer.rs:13-16). */
 typedef enum { SVL_NORM_LAYER = 0, SVL_NORM_RMS = 1 } svl_norm_kind;
 /* Weight storage. Q8_0 is what Linear::from_weight builds (nn/mod.rs:76-88); Q4_1 (32
- * 4-bit values with an f16 scale and min) has no reference counterpart. */
-typedef enum { SVL_DT_F32 = 0, SVL_DT_BF16 = 1, SVL_DT_Q8_0 = 2, SVL_DT_Q4_1 = 3 } svl_dtype;
+ * 4-bit values with an f16 scale and min) and F8 (e4m3 with an f32 scale per block of 128 x 128;
+ * activations as e4m3 rows with a scale per 128 columns, see svl_add_norm_f8_device) have no
+ * reference counterpart. F8 is for STT models without layer scale, for any number of streams;
+ * its states cannot be SVL_STATE_REFERENCE_ORDER (SVL_ERR_UNSUPPORTED). */
+typedef enum {
+  SVL_DT_F32 = 0,
+  SVL_DT_BF16 = 1,
+  SVL_DT_Q8_0 = 2,
+  SVL_DT_Q4_1 = 3,
+  SVL_DT_F8 = 4
+} svl_dtype;
 
 /* TransformerConfig (nn/transformer.rs:27-41). `quantize` becomes weight_dtype; context 0
  * means None (unlimited). kv_dtype is F32 (the reference CPU path) or BF16 (its CUDA path,
@@ -202,6 +211,28 @@ SVL_API svl_status svl_stt_run_frames(svl_model* model, svl_state* state, int32_
 SVL_API svl_status svl_stt_run_frames_ex(svl_model* model, svl_state* state, int32_t batch,
                                          int32_t n_frames, const uint32_t* audio_tokens,
                                          uint32_t* out_tokens, float* out_extra);
+
+/* Rules for the text tokens of a stream (or of all, stream < 0) of an STT state, host memory; they
+ * take effect with the next step and stay until they are set again. rules == NULL: none. No
+ * counterpart in the reference, whose Recognizer takes the argmax as it is. */
+#define SVL_RULES_HISTORY 1024 /* recorded tokens per stream: the last 1,024 */
+#define SVL_RULES_BIASES 256   /* biased tokens per stream, at most */
+typedef struct svl_stt_rules {
+  /* A token that occurs c > 0 times among the stream's recorded tokens: l > 0 ? l / repetition :
+   * l * repetition, then - (frequency * c + presence). 1, 0, 0 for none; repetition > 0. */
+  float repetition, frequency, presence;
+  /* Tokens below this id are neither recorded nor penalised (4: the padding tokens). */
+  int32_t first_penalised;
+  int32_t n_bias; /* hot words: bias_values[i] is added to the logit of bias_ids[i] */
+  const uint32_t* bias_ids;
+  const float* bias_values;
+  const uint32_t* allowed; /* bit v % 32 of word v / 32: token v may follow; NULL = every token */
+} svl_stt_rules;
+/* The logits that a step returns are those after the rules. A step that no token may follow
+ * yields token 0xFFFFFFFF, which the next step refuses as out of range. first_penalised is the
+ * state's: the last call's value holds for every stream. A reset stream's recorded tokens are
+ * forgotten, svl_state_copy copies them between states that both have rules. */
+SVL_API svl_status svl_state_set_rules(svl_state* state, int32_t stream, const svl_stt_rules* rules);
 
 /* Transformer::forward (nn/transformer.rs:139-154) of one stream over xs [t][d_model] (host,
  * in place), t >= 1: the prefill path. */
@@ -367,7 +398,9 @@ SVL_API svl_status svl_rvq_encode_device(svl_rvq* rvq, int32_t batch, int32_t fr
  *
  * e4m3 rows with one f32 scale per row and block of 128 columns: value (r, c) stands for
  * e4m3(d_q[r * q_stride + c]) * d_scales[(c / 128) * scale_stride + r]. They have no
- * counterpart in the reference, whose weights are f32, bf16 or Q8_0.
+ * counterpart in the reference, whose weights are f32, bf16 or Q8_0. An SVL_DT_F8 model runs its
+ * steps through these operators; svl_state_set_rules puts the rules behind the head of any STT
+ * model.
  *
  * `device` is the GPU that holds the tensors (it need not be the current one, which a call leaves
  * as it was), `cuda_stream` a stream of it (NULL = its default stream). Calls only enqueue work,

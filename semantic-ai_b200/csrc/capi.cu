@@ -163,6 +163,7 @@ SVL_API svl_status svl_state_copy(svl_state* to, int32_t dst, const svl_state* f
     // The stream's last argmax travels with it (the text token a resumed stream feeds back).
     if (a.tok_out.p && b.tok_out.p)
       svl::check_cuda(cudaMemcpyAsync(a.tok_out.as<uint32_t>() + dst, b.tok_out.as<uint32_t>() + src, 4, cudaMemcpyDeviceToDevice, st), "copy");
+    svl::state_copy_said(a, dst, b, src, st);
     a.hpos[dst] = b.hpos[src];
     svl::check_cuda(cudaMemcpyAsync(a.pos.as<int>() + dst, &a.hpos[dst], 4, cudaMemcpyHostToDevice, st), "copy");
     svl::check_cuda(cudaStreamSynchronize(st), "copy");
@@ -354,6 +355,17 @@ SVL_API svl_status svl_stt_run_frames_ex(svl_model* model, svl_state* state, int
     svl::check_cuda(cudaStreamSynchronize(st), "frames");
     for (int b = 0; b < batch; b++) s.hpos[b] += n_frames;
     svl::raise_device_error(s, st);
+  });
+}
+
+SVL_API svl_status svl_state_set_rules(svl_state* state, int32_t stream, const svl_stt_rules* rules) {
+  return guarded([&] {
+    need(state, SVL_ERR_INVALID_INPUT, "null state");
+    svl::State& s = *state->s;
+    need(s.m->kind == 0, SVL_ERR_INVALID_INPUT, "not an STT model");
+    if (stream >= 0) check_stream(s, stream);
+    svl::check_cuda(cudaSetDevice(s.m->device), "cudaSetDevice");
+    svl::state_set_rules(s, stream, rules);
   });
 }
 

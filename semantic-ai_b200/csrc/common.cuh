@@ -7,12 +7,13 @@
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 namespace svl {
 
-enum WeightType { W_F32 = 0, W_BF16 = 1, W_Q8 = 2, W_Q4 = 3 };
+enum WeightType { W_F32 = 0, W_BF16 = 1, W_Q8 = 2, W_Q4 = 3, W_F8 = 4 };
 enum NormKind { NORM_NONE = 0, NORM_RMS = 1, NORM_LAYER = 2 };
 
 constexpr int QBLK = 32;  // quantisation block (ggml QK8_0 / QK4_1)
@@ -87,5 +88,16 @@ __device__ __forceinline__ float round_bf16(float x) {
   return __bfloat162float(__float2bfloat16_rn(x));
 }
 __device__ __forceinline__ float f16_round(float x) { return __half2float(__float2half_rn(x)); }
+
+// The nearest e4m3 value (ties to even), at most 448.
+__device__ __forceinline__ uint8_t to_e4m3(float v) {
+  return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+}
+// Maximum that keeps a NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
 }  // namespace svl

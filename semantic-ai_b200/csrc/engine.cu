@@ -111,18 +111,35 @@ struct Loader {
   void linear(Linear& L, const std::string& wname, const std::string& bname, int n_out, int k,
               bool quantizable, int interleave = 0) {
     const svl_tensor_view& v = need(wname, (int64_t)n_out * k);
-    if (k % QBLK) throw Error(SVL_ERR_UNSUPPORTED, "linear " + wname + ": k % 32 != 0");
     int wt = W_F32;
     switch (m.cfg.weight_dtype) {
       case SVL_DT_BF16: wt = W_BF16; break;
       case SVL_DT_Q8_0: wt = quantizable ? W_Q8 : W_F32; break;
       case SVL_DT_Q4_1: wt = quantizable ? W_Q4 : W_F32; break;
+      case SVL_DT_F8: wt = quantizable ? W_F8 : W_F32; break;
       default: wt = W_F32;
     }
+    if (k % QBLK && wt != W_F8) throw Error(SVL_ERR_UNSUPPORTED, "linear " + wname + ": k % 32 != 0");
     L.n = n_out;
     L.k = k;
     L.wtype = wt;
     L.interleave = interleave;
+    if (wt == W_F8) {
+      // The rows in their own order (the activation kernel pairs them), 128 bytes per block.
+      L.interleave = 0;
+      L.f8.n = n_out;
+      L.f8.k = k;
+      L.row_stride = (int64_t)L.f8.kblocks() * kF8Block;
+      L.w.alloc((int64_t)L.f8.tiles() * L.f8.kblocks() * kF8TileBytes);
+      L.f8_scales.alloc((int64_t)L.f8.tiles() * L.f8.kblocks() * 4);
+      check_cuda(cudaMemsetAsync(L.w.p, 0, L.w.bytes, m.stream), "memset");
+      launch_f8_quantise(stage(v), n_out, k, L.w.as<uint8_t>(), L.f8_scales.as<float>(), m.stream);
+      check_cuda(cudaStreamSynchronize(m.stream), "pack weights");
+      L.f8.w = L.w.as<uint8_t>();
+      L.f8.scales = L.f8_scales.as<float>();
+      m.weight_bytes += L.row_stride * n_out + (int64_t)L.f8_scales.bytes;
+      return;
+    }
     L.row_stride = packed_row_stride(wt, k);
     L.w.alloc(L.row_stride * n_out);
     // Zero first: the unused blocks of a partial last super-block stay zero.
@@ -213,7 +230,7 @@ void validate_cfg(const svl_transformer_config& c) {
   if (c.d_model % 32) throw Error(SVL_ERR_UNSUPPORTED, "d_model must be a multiple of 32");
   if (c.ffn_kind < 0 || c.ffn_kind > 2) bad("unknown feed-forward kind");
   if (c.norm_kind < 0 || c.norm_kind > 1) bad("unknown norm kind");
-  if (c.weight_dtype < 0 || c.weight_dtype > 3) bad("unknown weight dtype");
+  if (c.weight_dtype < 0 || c.weight_dtype > SVL_DT_F8) bad("unknown weight dtype");
   if (c.kv_dtype < 0 || c.kv_dtype > 1) bad("unknown kv dtype");
   if (c.context < 0) bad("negative context");
   if (c.ffn_hidden <= 0) bad("non-positive ffn_hidden");
@@ -261,6 +278,8 @@ Model* create_model(int kind, const svl_transformer_config& cfg, const svl_stt_c
                     const svl_tts_config* tts, const svl_tensor_view* t, int n, int device,
                     const char* prefix) {
   validate_cfg(cfg);
+  if (cfg.weight_dtype == SVL_DT_F8 && (kind != 0 || cfg.layer_scale))
+    throw Error(SVL_ERR_UNSUPPORTED, "F8 weights are for STT models without layer scale");
   int count = 0;
   check_cuda(cudaGetDeviceCount(&count), "cudaGetDeviceCount");
   if (device < 0 || device >= count) throw Error(SVL_ERR_CUDA, "no such CUDA device");
@@ -409,6 +428,8 @@ constexpr int kRefRopePositions = 8192;
 
 State* create_state(Model* m, int max_batch, int max_positions, uint32_t flags) {
   if (max_batch <= 0) throw Error(SVL_ERR_INVALID_INPUT, "max_batch must be positive");
+  if (is_f8(*m) && (flags & SVL_STATE_REFERENCE_ORDER))
+    throw Error(SVL_ERR_UNSUPPORTED, "F8 models have no reference order");
   check_cuda(cudaSetDevice(m->device), "cudaSetDevice");
   const auto& c = m->cfg;
   State* s = new State();
@@ -512,6 +533,7 @@ State* create_state(Model* m, int max_batch, int max_positions, uint32_t flags) 
         if (!ok) throw Error(SVL_ERR_CUDA, "cannot encode the TMA tensor maps of the GEMM operands");
       }
     }
+    if (is_f8(*m)) create_state_f8(*m, *s);
     s->am_ticket.alloc(4);
     check_cuda(cudaMemsetAsync(s->am_ticket.p, 0, 4, m->stream), "memset");
     s->err.alloc(4);
@@ -764,6 +786,11 @@ LayerParams layer_params(Model& m, State& s, int l, int b0, int nb) {
 
 void enqueue_layers_mask(Model& m, State& s, int b0, int nb, cudaStream_t st, bool do_lin,
                          bool do_attn) {
+  if (is_f8(m)) {
+    enqueue_layers_f8(m, s, b0, nb, st, do_lin, do_attn);
+    if (do_lin) f8_flush(m, s, b0, nb, st);
+    return;
+  }
   const auto& c = m.cfg;
   const int d = c.d_model, hd = c.head_dim, qd = c.num_heads * hd;
   float* x = s.x.as<float>() + (int64_t)b0 * d;
@@ -847,6 +874,10 @@ GemvParams head_params(Model& m, State& s, int nb) {
 // The logits product with its argmax: on the tensor cores (out_norm as the operand prep)
 // when the step's products run there.
 void launch_head(Model& m, State& s, const GemvParams& g, cudaStream_t st) {
+  if (is_f8(m)) {
+    f8_head(m, s, g.nb, false, st);
+    return;
+  }
   if (use_tensor_cores(m, s, g.nb)) {
     const int d = m.cfg.d_model;
     launch_prep_bf16(g.x, d, g.nb, m.out_norm.kind, m.out_norm.w.as<float>(),
@@ -875,12 +906,20 @@ void enqueue_stt_step(Model& m, State& s, int nb, cudaStream_t st) {
   e.x = s.x.as<float>();
   e.error_flag = s.err.as<int>();
   launch_embed(e, st);
-  enqueue_layers(m, s, 0, nb, st);
-  // out_norm + text_linear + argmax (stt/model.rs:252-258). The step's last reader of the
-  // positions is done once the argmax is final: the argmax's last CTA advances them.
-  GemvParams g = head_params(m, s, nb);
-  g.pos_advance = s.pos.as<int>();
-  launch_head(m, s, g, st);
+  if (is_f8(m)) {
+    enqueue_layers_f8(m, s, 0, nb, st, true, true);
+    f8_head(m, s, nb, true, st);
+    enqueue_rules(m, s, nb, st);
+    launch_advance_positions(s.pos.as<int>(), nb, st);
+  } else {
+    enqueue_layers(m, s, 0, nb, st);
+    // out_norm + text_linear + argmax (stt/model.rs:252-258). The step's last reader of the
+    // positions is done once the argmax is final: the argmax's last CTA advances them.
+    GemvParams g = head_params(m, s, nb);
+    g.pos_advance = s.pos.as<int>();
+    launch_head(m, s, g, st);
+    if (s.rules) enqueue_rules(m, s, nb, st);
+  }
   // Extra (VAD) heads: softmax p[0] of each (stt/model.rs:259-271); never quantised.
   const int eh = m.stt.extra_heads_num, edim = m.stt.extra_heads_dim;
   for (int i = 0; i < eh; i++) {
@@ -1131,6 +1170,7 @@ void state_reset(State& s, int stream) {
   check_cuda(cudaMemcpyAsync(s.pos.as<int>() + b0, s.hpos.data() + b0, (b1 - b0) * 4,
                              cudaMemcpyHostToDevice, s.m->stream),
              "reset");
+  if (s.rules) check_cuda(cudaMemsetAsync(s.said_len.as<int>() + b0, 0, (b1 - b0) * 4, s.m->stream), "reset");
   check_cuda(cudaStreamSynchronize(s.m->stream), "reset");
 }
 

@@ -15,6 +15,7 @@
 
 #include "../../include/svl_cuda.h"
 #include "common.cuh"
+#include "f8.cuh"
 #include "kernels.cuh"
 
 namespace svl {
@@ -61,6 +62,8 @@ struct Linear {
   DevBuf bias;  // f32 [n] or empty
   GemmOperand tc;  // TMA map of the bf16 weights for the tensor-core path
   DevBuf shadow;   // Q8_0 / Q4_1: the bf16 image of the dequantised weights (tensor cores)
+  DevBuf f8_scales;  // F8: the blocks' scales; w is the packed image
+  F8Matrix f8;
   int64_t bytes() const { return row_stride * n + (bias.p ? 4LL * n : 0); }
 };
 
@@ -170,6 +173,13 @@ struct State {
   DevBuf rope_tab;         // [rope_positions][head_dim / 2] (cos, sin)
   int rope_positions = 0;
   bool test_withheld_copy = false;  // SVL_STATE_TEST_WITHHELD_COPY: the bounded-wait drill
+  // F8 weights: e4m3 rows and their scales (the operand of the next product), a product's f32
+  // outputs before RoPE or the activation, and the block outputs that the next norm adds to x.
+  DevBuf f8_q, f8_s, f8_y, f8_delta;
+  // Rules between logits and token (svl_state_set_rules), once they have been set.
+  bool rules = false;
+  int rules_first = 0;
+  DevBuf said, said_len, rule_rep, rule_freq, rule_pres, rule_ids, rule_vals, rule_masks, rule_rows;
   ~State();
 };
 
@@ -178,6 +188,8 @@ struct LayerParams {
   GemvParams in_proj, out_proj, ff1, ff2;
   AttnParams attn;
 };
+
+LayerParams layer_params(Model& m, State& s, int l, int b0, int nb);
 
 // Streams from which a step's weight products run on the tensor cores (bf16 weights).
 constexpr int kGemmMinBatch = 16;
@@ -213,11 +225,22 @@ int capture_tts_graph(Model& m, State& s, int nb, int decode_steps, cudaStream_t
 // device tokens [nb][n].
 void enqueue_tts_prompt(Model& m, State& s, int b0, int nb, const uint32_t* d_tokens, int n,
                         cudaStream_t st);
+// F8 models (f8_step.cu). The layers of streams [b0, b0 + nb): the last block's output stays in
+// s.f8_delta until f8_flush adds it to x, or the head's norm does (f8_head with `pending`).
+inline bool is_f8(const Model& m) { return m.cfg.weight_dtype == SVL_DT_F8; }
+void create_state_f8(Model& m, State& s);
+void enqueue_layers_f8(Model& m, State& s, int b0, int nb, cudaStream_t st, bool do_lin, bool do_attn);
+void f8_flush(Model& m, State& s, int b0, int nb, cudaStream_t st);
+void f8_head(Model& m, State& s, int nb, bool pending, cudaStream_t st);
+// The rules of streams [0, nb) on s.logits in place, and their picks into s.tok_out.
+void enqueue_rules(Model& m, State& s, int nb, cudaStream_t st);
 // Profiling: one repetition of the step's weight products (which 0) or attention (which 1).
 int64_t enqueue_profile(Model& m, State& s, int nb, int which, cudaStream_t st);
 void enqueue_tts_step(Model& m, State& s, int nb, int decode_steps, bool bos, cudaStream_t st);
 
 void state_reset(State& s, int stream);
+void state_set_rules(State& s, int stream, const svl_stt_rules* rules);
+void state_copy_said(State& to, int dst, const State& from, int src, cudaStream_t st);
 // Message of the last failure on this thread (svl_last_error).
 void set_last_error(const std::string& msg);
 void state_export(State& s, int stream, int layer, float* k, float* v, int* len);

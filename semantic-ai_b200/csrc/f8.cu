@@ -1,7 +1,6 @@
 // f8.cu — e4m3 rows with a scale per 128 columns: the norm that writes them and the product
 // that reads them.
 #include <algorithm>
-#include <cuda_fp8.h>
 #include <memory>
 #include <string>
 
@@ -12,16 +11,6 @@
 
 namespace svl {
 namespace {
-
-__device__ __forceinline__ uint8_t to_e4m3(float v) {
-  return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
-}
-// Maximum that keeps a NaN.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 
 // V consecutive values of a row as they lie in memory; `have` of them exist. `wide`: the row starts
 // on 16 bytes.
@@ -233,15 +222,13 @@ __global__ void f8_pack_kernel(const uint8_t* src, int64_t stride, int n, int k,
 }
 
 // One CTA per 128 x 128 block: its largest magnitude, its scale, its e4m3 values.
-__global__ void __launch_bounds__(256) f8_quantise_kernel(const float* src, int n, int k, int half, uint8_t* dst,
-                                                          float* scales) {
+__global__ void __launch_bounds__(256) f8_quantise_kernel(const float* src, int n, int k, uint8_t* dst, float* scales) {
   __shared__ float red[8];
   const int kb = blockIdx.x, tile = blockIdx.y, kblocks = gridDim.x;
   auto value = [&](int i) -> float {
     const int r = tile * kF8Block + i / kF8Block, c = kb * kF8Block + i % kF8Block;
     if (r >= n || c >= k) return 0.f;
-    const int sr = half ? (r & 1) * half + (r >> 1) : r;
-    return src[(int64_t)sr * k + c];
+    return src[(int64_t)r * k + c];
   };
   float top = 0.f;
   for (int i = threadIdx.x; i < kF8Block * kF8Block; i += 256) top = max_nan(top, fabsf(value(i)));
@@ -339,10 +326,9 @@ void launch_f8_pack(const uint8_t* src, int64_t stride, int n, int k, uint8_t* d
   check_cuda(cudaGetLastError(), "pack launch");
 }
 
-void launch_f8_quantise(const float* src, int n, int k, int interleave_half, uint8_t* dst, float* scales,
-                        cudaStream_t s) {
+void launch_f8_quantise(const float* src, int n, int k, uint8_t* dst, float* scales, cudaStream_t s) {
   const dim3 grid((k + kF8Block - 1) / kF8Block, (n + kF8Block - 1) / kF8Block);
-  f8_quantise_kernel<<<grid, 256, 0, s>>>(src, n, k, interleave_half, dst, scales);
+  f8_quantise_kernel<<<grid, 256, 0, s>>>(src, n, k, dst, scales);
   check_cuda(cudaGetLastError(), "quantise launch");
 }
 
@@ -457,7 +443,7 @@ SVL_API svl_status svl_f8_linear_create(int32_t n, int32_t k, const svl_tensor_v
     svl::DevBuf staging;
     staging.alloc((size_t)n * k * 4);
     svl::check_cuda(cudaMemcpyAsync(staging.p, weight->data, staging.bytes, cudaMemcpyHostToDevice, st), "upload");
-    svl::launch_f8_quantise(staging.as<float>(), n, k, 0, L->w.as<uint8_t>(), L->scales.as<float>(), st);
+    svl::launch_f8_quantise(staging.as<float>(), n, k, L->w.as<uint8_t>(), L->scales.as<float>(), st);
     if (bias) svl::check_cuda(cudaMemcpyAsync(L->bias.p, bias->data, (size_t)n * 4, cudaMemcpyHostToDevice, st), "upload");
     svl::check_cuda(cudaStreamSynchronize(st), "create");
     *out = L.release();

@@ -49,10 +49,8 @@ constexpr int64_t kF8TileBytes = (int64_t)kF8Block * kF8Block;
 
 // Packs row-major e4m3 rows (stride bytes apart) into a zeroed image.
 void launch_f8_pack(const uint8_t* src, int64_t stride, int n, int k, uint8_t* dst, cudaStream_t s);
-// Quantises f32 [n][k] (packed row 2i taken from row i and 2i+1 from row interleave_half + i when
-// that is set) into a zeroed image and its scales.
-void launch_f8_quantise(const float* src, int n, int k, int interleave_half, uint8_t* dst,
-                        float* scales, cudaStream_t s);
+// Quantises f32 [n][k] into a zeroed image and its scales.
+void launch_f8_quantise(const float* src, int n, int k, uint8_t* dst, float* scales, cudaStream_t s);
 
 struct F8GemmParams {
   F8Matrix m;

@@ -63,6 +63,8 @@ extern "C" SVL_API svl_status svl_stt_head_noalloc(svl_model* model, int32_t bat
       throw Error(SVL_ERR_INVALID_INPUT,
                   "svl_stt_head_noalloc: batch must be 1..8 (its fixed scratch holds the "
                   "argmax candidates of 8 streams); call it once per group of 8 streams");
+    if (svl::is_f8(m))
+      throw Error(SVL_ERR_UNSUPPORTED, "svl_stt_head_noalloc: an F8 head needs a state's buffers");
     svl::check_cuda(cudaSetDevice(m.device), "cudaSetDevice");
     unsigned char* scratch = scratch_on(m.device);
     cudaStream_t st = cuda_stream ? static_cast<cudaStream_t>(cuda_stream) : m.stream;

@@ -54,6 +54,7 @@ SIGNATURES = {
     "svl_profile_kernels": (_I, [_P, _P, _I, _I, _I, _P, ctypes.POINTER(ctypes.c_int64)]),
     "svl_step_kernel_count": (_I, [_P, _P, _I, ctypes.POINTER(ctypes.c_int32)]),
     "svl_state_error": (_I, [_P]),
+    "svl_state_set_rules": (_I, [_P, _I, _P]),
     "svl_stt_head_noalloc": (_I, [_P, _I, _P, _P, _P, _P]),
     "svl_mimi_create": (_I, [_P, _P, _I, _I, ctypes.POINTER(_P)]),
     "svl_mimi_destroy": (None, [_P]),

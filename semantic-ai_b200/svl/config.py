@@ -13,7 +13,7 @@ from dataclasses import dataclass, replace
 
 FFN_PLAIN_GELU_TANH, FFN_PLAIN_GELU_ERF, FFN_GATED_SILU = 0, 1, 2
 NORM_LAYER, NORM_RMS = 0, 1
-DTYPES = {"f32": 0, "bf16": 1, "q8_0": 2, "q4_1": 3}
+DTYPES = {"f32": 0, "bf16": 1, "q8_0": 2, "q4_1": 3, "f8": 4}
 FLOW_KINDS = {"lsd": 0, "flow_matching": 1, "drifting": 2, "pointwise": 3}
 
 

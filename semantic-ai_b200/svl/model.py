@@ -34,6 +34,14 @@ def tensor_views(tensors: dict[str, np.ndarray]):
     return views, keep
 
 
+class CSttRules(ctypes.Structure):
+    """svl_stt_rules (include/svl_cuda.h)."""
+    _fields_ = [("repetition", ctypes.c_float), ("frequency", ctypes.c_float), ("presence", ctypes.c_float),
+                ("first_penalised", ctypes.c_int32), ("n_bias", ctypes.c_int32),
+                ("bias_ids", ctypes.POINTER(ctypes.c_uint32)), ("bias_values", ctypes.POINTER(ctypes.c_float)),
+                ("allowed", ctypes.POINTER(ctypes.c_uint32))]
+
+
 class State:
     """Per-stream KV rings and positions for up to max_batch streams."""
 
@@ -84,6 +92,38 @@ class State:
             shape = (c.num_kv_heads, n.value, c.head_dim)
             out.append((k[: np.prod(shape)].reshape(shape), v[: np.prod(shape)].reshape(shape)))
         return out
+
+    def set_rules(self, stream: int = -1, repetition: float = 1.0, frequency: float = 0.0, presence: float = 0.0,
+                  first_penalised: int = 4, bias: dict | None = None, allowed=None):
+        """Rules for the text tokens of one stream, or of all (svl_state_set_rules): penalties for
+        tokens that the stream has said (ids from first_penalised on), `bias` {token: value} for hot
+        words, and `allowed`, the tokens that may follow (ids, or a truth value per token)."""
+        bias = bias or {}
+        ids = np.array(list(bias.keys()), np.uint32)
+        vals = np.array(list(bias.values()), np.float32)
+        bits = None
+        if allowed is not None:
+            card = self.model.stt.text_card
+            a = np.asarray(allowed)
+            if a.dtype == bool:
+                if a.shape != (card,):
+                    raise ValueError(f"allowed must have {card} truth values: got {a.shape}")
+                ok = a
+            else:
+                if a.size and (a.min() < 0 or a.max() >= card):
+                    raise ValueError(f"allowed tokens must be below {card}")
+                ok = np.zeros(card, bool)
+                ok[a.astype(np.int64)] = True
+            padded = np.zeros((card + 31) // 32 * 32, np.uint8)
+            padded[:card] = ok
+            bits = np.packbits(padded, bitorder="little").view(np.uint32)
+        r = CSttRules(repetition, frequency, presence, first_penalised, len(ids), _u32(ids), _f32(vals),
+                      None if bits is None else _u32(bits))
+        _lib.check(_lib.lib().svl_state_set_rules(self.handle, stream, ctypes.byref(r)))
+
+    def clear_rules(self, stream: int = -1):
+        """No rules for one stream, or for all."""
+        _lib.check(_lib.lib().svl_state_set_rules(self.handle, stream, None))
 
     def save_voice(self, path, stream: int = 0):
         """Voice::save (tts/voice.rs:78-99): this stream's KV state as a safetensors voice."""

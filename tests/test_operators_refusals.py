@@ -97,3 +97,9 @@ def test_python_checks_come_first():
         svl.F8Linear(cpu, cpu)
     with pytest.raises(ValueError, match="logits must be a CUDA tensor"):
         svl.logits_rules(cpu)
+
+
+def test_state_rules_refuse_without_a_state(svl_lib):
+    from svl import _lib
+    with pytest.raises(_lib.SvlError, match="null state"):
+        _lib.check(svl_lib.svl_state_set_rules(None, -1, None))
