@@ -1,6 +1,7 @@
 // rules.cu — the rules between logits and token: penalties for repeated tokens, biases, grammar
 // masks, and the greedy pick.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "common.cuh"
@@ -16,6 +17,13 @@ __device__ __forceinline__ float load_logit(const __nv_bfloat16* p) { return __b
 __device__ __forceinline__ void store_logit(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_logit(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
+// 16 bytes that are read once.
+__device__ __forceinline__ uint4 load_once(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
+
 // An order-preserving key of a value above -infinity (0: none), then the lowest index: the
 // larger key wins.
 __device__ __forceinline__ uint64_t pick_key(float v, int i) {
@@ -26,33 +34,46 @@ __device__ __forceinline__ uint64_t pick_key(float v, int i) {
 }
 __device__ __forceinline__ uint64_t max_key(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
-constexpr int kMaxThreads = 1024;
-constexpr int kMaxChunk = 16384;  // tokens whose counts are held at once: 64 KB
+constexpr int kMaxChunk = 131104;      // tokens of a CTA's chunk at most: 131,072 and the lead
+constexpr int kMaxChunkLong = 16416;   // the same with lists of more than kLongLists entries
+constexpr int kLongLists = 8192;
+constexpr int kDirect = 8192;          // tokens of a chunk that has counts for all of them
 constexpr int kAhead = 4;         // 16-byte loads of logits a thread has in flight
-constexpr int kListAhead = 8;     // history entries a thread has in flight
-constexpr int kMaxTouched = 4096; // touched tokens of a chunk that are listed (more are searched for)
+constexpr int kSettle = 2;        // touched tokens whose logits a thread has in flight over the stream
+constexpr int kSlotBytes = 12;    // a touched token's count, first bias entry and position
 
 // Bound by HBM for many tokens, by a chain of a few dependent loads for few. A row is shared by the
 // CTAs of a cluster, each with a contiguous range of the vocabulary, taken in chunks (one, up to
 // 131,072 tokens in 8 CTAs).
 //
-// The lists touch few tokens, so they are settled first and the stream over all tokens stays
-// short (about ten instructions per token): `word` counts each token in the history (low 16 bits)
-// and holds its first entry in the sparse biases (65,535 minus its index, high 16), by atomics whose
-// result does not depend on their order. The entry that finds a token's word empty puts the token
-// on a list and sets its bit in `touched`; then one thread per listed token computes its value up
-// to the grammar and leaves it in `word`. The stream takes touched tokens' values from there. The
-// row's first logits and history entries are on their way meanwhile.
+// The lists touch few tokens, so these are kept out of the stream over all tokens: each sets a bit in
+// `touched`; then every word of bits takes as many slots as it has bits (a token's slot is its word's
+// first plus the bits below its own), where the history counts the token and the sparse biases leave
+// their first entry, by atomics whose result does not depend on their order. The touched tokens'
+// logits are fetched before the stream, which passes over them as it does over tokens that the
+// grammar forbids, and written after it. The row's first logits and list entries are on their way
+// meanwhile. A chunk of at most 8,192 tokens has a count and an entry for each (`direct`): zeroing them
+// takes less than giving slots (256 rows of 4,001 f32 tokens with all rules: 10.4 us, 11.3 with
+// slots).
+//
+// Measured: 1 row of 8,000 f32 tokens with a history of 250, 16 biases and a mask 5.7 us (2.8 without
+// rules); 256 rows of 4,001 f32 with all rules 8.9 us; 192 rows of 131,072 bf16 with all rules, a
+// history of 2,048 each, 50 us, of which half is the copy: 2.1 TB/s. More warps per SM would hide
+// more of the lists' latency, but below 64 registers the spills cost more than they bring.
 //
 // Positions are counted from the 16-byte boundary at or before the row's start ("lead" elements
 // before it), so that every row is read in aligned 16-byte pieces, also where rows of an odd
-// vocabulary start anywhere.
-template <class T>
-__global__ void __launch_bounds__(kMaxThreads) rules_kernel(const __grid_constant__ RulesParams p, int split, int range,
-                                                            int chunk) {
+// vocabulary start anywhere; the elements before the first and after the last whole piece are
+// taken one by one. The stream remembers the raw piece of its largest value; which of the piece's
+// tokens it was is looked up once, at the end.
+template <class T, int Threads, int PerSm>
+__global__ void __launch_bounds__(Threads, PerSm) rules_kernel(const __grid_constant__ RulesParams p, int split, int range,
+                                                               int chunk, int slots, int direct) {
   constexpr int VE = 16 / sizeof(T);
-  extern __shared__ uint32_t word[];  // [chunk], then the bits
-  __shared__ uint64_t best_sm[kMaxThreads / 32], best_of[8];
+  constexpr int kListAhead = 2048 / Threads;  // history entries a thread has in flight
+  extern __shared__ __align__(16) uint32_t count[];  // [slots]; then a settled value, past the threads' own
+  __shared__ uint64_t best_sm[Threads / 32], best_of[8];
+  __shared__ float penalty[3];  // repetition, frequency, presence
   __shared__ int twice, touched_n;
   const svl_logits_rules& R = p.rules;
   const int t = threadIdx.x, threads = blockDim.x;
@@ -61,34 +82,18 @@ __global__ void __launch_bounds__(kMaxThreads) rules_kernel(const __grid_constan
   if (split > 1) cluster_arrive();  // waited for before the ranks' shared memory is written
   pdl_launch();
   pdl_wait();
-  uint32_t* touched = word + chunk;  // [chunk / 32], then the list
-  uint16_t* list = reinterpret_cast<uint16_t*>(touched + chunk / 32);
+  uint32_t* first = count + slots;  // 65,536 minus the first entry's index, 0: none
+  int* list = reinterpret_cast<int*>(first + slots);
+  uint32_t* touched = first + 2 * slots;       // [chunk / 32]
+  uint32_t* word_slot = touched + chunk / 32;  // [chunk / 32]
   const T* in = static_cast<const T*>(p.logits) + r * p.logits_stride;
   T* out = p.out ? static_cast<T*>(p.out) + r * p.out_stride : nullptr;
   const int lead = (int)(reinterpret_cast<uintptr_t>(in) % 16 / sizeof(T));
   const bool wide_out = out && (reinterpret_cast<uintptr_t>(out) - reinterpret_cast<uintptr_t>(in)) % 16 == 0;
   const float* dense = R.d_dense_bias;
   const bool wide_bias = lead == 0 && reinterpret_cast<uintptr_t>(dense) % 16 == 0;
-  const int end = p.vocab + lead;
+  const int end = p.vocab + lead, whole = end / VE * VE;  // whole: the end of the last whole piece
   const int lo = rank * range, hi = min(lo + range, end);
-
-  // 16 bytes of logits at position u (a multiple of VE), in flight until they are read.
-  auto load = [&](int u) {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    const T* src = in - lead + u;
-    if (u >= lead && u + VE <= end) {
-      asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                   : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                   : "l"(src)
-                   : "memory");
-    } else {
-      T e[VE];
-#pragma unroll
-      for (int j = 0; j < VE; j++) e[j] = u + j >= lead && u + j < end ? src[j] : T(0.f);
-      v = *reinterpret_cast<uint4*>(e);
-    }
-    return v;
-  };
 
   const int32_t* hist = R.d_history ? R.d_history + r * R.history_stride : nullptr;
   const int said = R.d_history ? max(0, min(R.d_lengths[r], R.history_cap)) : 0;
@@ -100,178 +105,236 @@ __global__ void __launch_bounds__(kMaxThreads) rules_kernel(const __grid_constan
   const int listed = R.d_bias_ids ? R.bias_cap : 0;
   const int32_t* ids = listed ? R.d_bias_ids + r * R.bias_stride : nullptr;
   const float* vals = listed ? R.d_bias_values + r * R.bias_stride : nullptr;
+  const int bias_id = t < listed ? ids[t] : -1;
   const uint32_t* mask = nullptr;
   if (R.d_masks) {
     const int64_t m = R.d_mask_rows ? R.d_mask_rows[r] : r;
     if (m >= 0 && m < R.n_masks) mask = R.d_masks + m * R.mask_stride;
   }
-  float bv = -INFINITY;
-  int bi = 0;
+  if (t < 3) {  // there are barriers before a counted token is settled
+    const float* per_row = t == 0 ? R.d_repetition : t == 1 ? R.d_frequency : R.d_presence;
+    penalty[t] = per_row ? per_row[r] : t == 0 ? 1.f : 0.f;
+  }
+  uint64_t best = 0;
   for (int c0 = lo; c0 < hi; c0 += chunk) {
     const int c1 = min(c0 + chunk, hi);
+    const int v0 = c0 - lead;  // position 0's token, below 0 before the row
+    // The chunk's whole pieces: c0 is a multiple of 32.
+    const int w0 = c0 == 0 && lead ? VE : c0, w1 = min(c1, whole);
     const int step = threads * VE;
     uint4 raw[kAhead];
 #pragma unroll
     for (int j = 0; j < kAhead; j++) {
-      const int u = c0 + j * step + t * VE;
-      if (u < c1) raw[j] = load(u);
+      const int u = w0 + j * step + t * VE;
+      if (u < w1) raw[j] = load_once(in - lead + u);
+    }
+    // The elements outside whole pieces, of one thread each.
+    int edge = -1;
+    if (t < VE && c0 == 0 && t >= lead && t < min(w0, end)) edge = t;
+    if (t >= VE && t < 2 * VE && max(whole, w0) + t - VE >= c0 && max(whole, w0) + t - VE < c1) edge = max(whole, w0) + t - VE;
+    float edge_l = 0.f, edge_dense = 0.f;
+    uint32_t edge_mask = ~0u;
+    if (edge >= 0) {
+      edge_l = load_logit(in - lead + edge);
+      if (dense) edge_dense = dense[edge - lead];
+      if (mask) edge_mask = mask[(edge - lead) >> 5];
     }
     const bool table = said || listed;
+    int n = 0;  // touched tokens
+    float mine[kSettle], mine_dense[kSettle];
+    // A touched token's value up to the grammar, of its logit and dense bias.
+    auto settled = [&](int i, float l, float d) {
+      const int at = direct ? list[i] : i;
+      const uint32_t c = count[at], f = first[at];
+      if (c) {
+        l = l > 0.f ? __fdiv_rn(l, penalty[0]) : l * penalty[0];
+        l = l - (penalty[1] * (float)c + penalty[2]);
+      }
+      if (dense) l = l + d;
+      if (f) {
+        const int entry = 65536 - (int)f;
+        l = l + vals[entry];
+        if (twice) {
+          const int v = v0 + list[i];
+          for (int k = entry + 1; k < listed; k++)
+            if (ids[k] == v) l = l + vals[k];
+        }
+      }
+      return l;
+    };
     if (table) {
-      const int v0 = c0 - lead;                         // position 0's token, below 0 before the row
       const int from = max(v0, 0), to = c1 - lead;      // the chunk's tokens
       const int floor = max(from, R.first_penalised);   // those that the history counts for
       __syncthreads();
-      for (int i = t * 4; i < (c1 - c0 + 31) / 32 * 32; i += threads * 4) *reinterpret_cast<uint4*>(word + i) = make_uint4(0, 0, 0, 0);
       for (int i = t; i < chunk / 32; i += threads) touched[i] = 0;
+      if (direct)  // slots is the chunk, a multiple of 32
+        for (int i = t * 4; i < 2 * slots; i += threads * 4) *reinterpret_cast<uint4*>(count + i) = make_uint4(0, 0, 0, 0);
       if (t == 0) twice = touched_n = 0;
       __syncthreads();
-      // Lists a token of the chunk, once per token.
-      auto touch = [&](int at) {
-        atomicOr(&touched[at >> 5], 1u << (at & 31));
-        const int n = atomicAdd(&touched_n, 1);
-        if (n < kMaxTouched) list[n] = (uint16_t)at;
-      };
-      if (listed) {
+      auto entries = [&](auto&& biased, auto&& repeated) {
         for (int i = t; i < listed; i += threads) {
-          const int id = ids[i];
-          if (id >= from && id < to) atomicMax(&word[id - v0], (uint32_t)(65535 - i) << 16);
+          const int id = i == t ? bias_id : ids[i];
+          if (id >= from && id < to) biased(i, id - v0);
+        }
+#pragma unroll
+        for (int j = 0; j < kListAhead; j++)
+          if (t + j * threads < said && said_id[j] >= floor && said_id[j] < to) repeated(said_id[j] - v0);
+        for (int i = t + kListAhead * threads; i < said; i += threads) {
+          const int id = hist[i];
+          if (id >= floor && id < to) repeated(id - v0);
+        }
+      };
+      // Sets a token's bit; true for the thread that found it unset. Most entries repeat a few tokens,
+      // so it looks before the atomic.
+      auto touch = [&](int at) {
+        const uint32_t bit = 1u << (at & 31);
+        if (*reinterpret_cast<volatile uint32_t*>(&touched[at >> 5]) & bit) return false;
+        return !(atomicOr(&touched[at >> 5], bit) & bit);
+      };
+      if (direct) {
+        auto add = [&](int at) {
+          if (touch(at)) list[atomicAdd(&touched_n, 1)] = at;
+        };
+        entries([&](int i, int at) { add(at); if (atomicMax(&first[at], 65536u - i)) twice = 1; },
+                [&](int at) { add(at); atomicAdd(&count[at], 1u); });
+        __syncthreads();
+      } else {
+        entries([&](int, int at) { touch(at); }, [&](int at) { touch(at); });
+        __syncthreads();
+        for (int w = t; w < chunk / 32; w += threads) {
+          uint32_t bits = touched[w];
+          if (!bits) continue;
+          int i = atomicAdd(&touched_n, __popc(bits));
+          word_slot[w] = i;
+          for (; bits; bits &= bits - 1, i++) {
+            list[i] = w * 32 + __ffs((int)bits) - 1;
+            count[i] = first[i] = 0;
+          }
         }
         __syncthreads();
-        for (int i = t; i < listed; i += threads) {
-          const int id = ids[i];
-          if (id < from || id >= to) continue;
-          if ((int)(word[id - v0] >> 16) == 65535 - i)
-            touch(id - v0);
-          else
-            twice = 1;
-        }
+        auto slot = [&](int at) { return word_slot[at >> 5] + __popc(touched[at >> 5] & ((1u << (at & 31)) - 1)); };
+        entries([&](int i, int at) { if (atomicMax(&first[slot(at)], 65536u - i)) twice = 1; },
+                [&](int at) { atomicAdd(&count[slot(at)], 1u); });
       }
-      for (int i0 = t; i0 < said; i0 += threads * kListAhead) {
-        if (i0 != t) {
+      n = touched_n;
 #pragma unroll
-          for (int j = 0; j < kListAhead; j++) said_id[j] = i0 + j * threads < said ? hist[i0 + j * threads] : -1;
-        }
-#pragma unroll
-        for (int j = 0; j < kListAhead; j++) {
-          const int id = said_id[j];
-          if (i0 + j * threads < said && id >= floor && id < to && atomicAdd(&word[id - v0], 1u) == 0) touch(id - v0);
-        }
+      for (int j = 0; j < kSettle; j++) {
+        const int i = t + j * threads;
+        mine[j] = i < n ? load_logit(in + v0 + list[i]) : 0.f;
+        mine_dense[j] = dense && i < n ? dense[v0 + list[i]] : 0.f;
       }
       __syncthreads();
-      const float rep = R.d_repetition ? R.d_repetition[r] : 1.f;
-      const float freq = R.d_frequency ? R.d_frequency[r] : 0.f, pres = R.d_presence ? R.d_presence[r] : 0.f;
-      auto settle = [&](int at) {
-        const int v = v0 + at;
-        const uint32_t w = word[at], c = w & 65535;
-        float l = load_logit(in + v);
-        if (c) {
-          l = l > 0.f ? __fdiv_rn(l, rep) : l * rep;
-          l = l - (freq * (float)c + pres);
+      if (n > kSettle * threads) {
+        for (int i = t + kSettle * threads; i < n; i += threads) {
+          const int v = v0 + list[i];
+          count[direct ? list[i] : i] = __float_as_uint(settled(i, load_logit(in + v), dense ? dense[v] : 0.f));
         }
-        if (dense) l = l + dense[v];
-        if (w >> 16) {
-          const int first = 65535 - (int)(w >> 16);
-          l = l + vals[first];
-          if (twice)
-            for (int k = first + 1; k < listed; k++)
-              if (ids[k] == v) l = l + vals[k];
-        }
-        word[at] = __float_as_uint(l);
-      };
-      const int n = touched_n;
-      if (n <= kMaxTouched) {
-        for (int i = t; i < n; i += threads) settle(list[i]);
-      } else {
-        for (int i = t; i < chunk / 32; i += threads)
-          for (uint32_t bits = touched[i]; bits; bits &= bits - 1) settle(i * 32 + __ffs((int)bits) - 1);
+        __syncthreads();  // the stream may overwrite the logits
       }
-      // The next chunk's first entries again, where there is one.
-      if (c1 < hi) {
-#pragma unroll
-        for (int j = 0; j < kListAhead; j++) said_id[j] = t + j * threads < said ? hist[t + j * threads] : -1;
-      }
-      __syncthreads();
     }
-    for (int u0 = c0 + t * VE; u0 < c1; u0 += kAhead * step) {
-      if (u0 >= c0 + kAhead * step) {
+    if (edge >= 0) {
+      const int v = edge - lead;
+      if (dense) edge_l = edge_l + edge_dense;
+      if ((n && touched[(edge - c0) >> 5] >> ((edge - c0) & 31) & 1) || !(edge_mask >> (v & 31) & 1)) edge_l = -INFINITY;
+      if (out) store_logit(out + v, edge_l);
+      best = max_key(best, pick_key(edge_l, v));
+    }
+    // A piece's values; those of touched and forbidden tokens are -infinity.
+    auto values = [&](const uint4& piece, int u, float* l) {
+      T e[VE];
+      *reinterpret_cast<uint4*>(e) = piece;
+      const int v = u - lead;
 #pragma unroll
-        for (int j = 0; j < kAhead; j++)
-          if (u0 + j * step < c1) raw[j] = load(u0 + j * step);
+      for (int i = 0; i < VE; i++) l[i] = load_logit(e + i);
+      if (dense) {
+        if (wide_bias) {
+#pragma unroll
+          for (int i = 0; i < VE; i += 4) {
+            const float4 d = __ldg(reinterpret_cast<const float4*>(dense + v + i));
+            l[i] = l[i] + d.x; l[i + 1] = l[i + 1] + d.y; l[i + 2] = l[i + 2] + d.z; l[i + 3] = l[i + 3] + d.w;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < VE; i++) l[i] = l[i] + __ldg(dense + v + i);
+        }
+      }
+      if (mask || n) {
+        uint32_t allowed = ~0u;
+        if (mask && !lead) {
+          allowed = __ldg(reinterpret_cast<const uint8_t*>(mask) + (v >> 3)) >> (v & 4);
+        } else if (mask) {
+          const int at = v >> 5, sh = v & 31;
+          const uint32_t low = __ldg(mask + at);
+          const uint32_t high = sh + VE > 32 ? __ldg(mask + at + 1) : 0u;
+          allowed = __funnelshift_r(low, high, sh);
+        }
+        if (n) allowed &= ~(touched[(u - c0) >> 5] >> ((u - c0) & 31));
+#pragma unroll
+        for (int i = 0; i < VE; i++)
+          if (!(allowed >> i & 1)) l[i] = -INFINITY;
+      }
+    };
+    float bv = -INFINITY;
+    int bu = -1;
+    uint4 piece = make_uint4(0, 0, 0, 0);
+    for (int b0 = w0; b0 < w1; b0 += kAhead * step) {
+      if (b0 != w0) {
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+          const int u = b0 + j * step + t * VE;
+          if (u < w1) raw[j] = load_once(in - lead + u);
+        }
       }
 #pragma unroll
       for (int j = 0; j < kAhead; j++) {
-        const int u = u0 + j * step;
-        if (u >= c1) break;
-        const int v = u - lead;  // the piece's first token (below 0 before the row)
-        T e[VE];
-        *reinterpret_cast<uint4*>(e) = raw[j];
+        const int u = b0 + j * step + t * VE;
+        if (u >= w1) continue;
         float l[VE];
+        values(raw[j], u, l);
+        if (out) {
+          T e[VE];
 #pragma unroll
-        for (int i = 0; i < VE; i++) l[i] = load_logit(e + i);
-        const bool inside = v >= 0 && v + VE <= p.vocab;
-        if (dense) {
-          if (wide_bias && inside) {
-#pragma unroll
-            for (int i = 0; i < VE; i += 4) {
-              const float4 d = __ldg(reinterpret_cast<const float4*>(dense + v + i));
-              l[i] = l[i] + d.x; l[i + 1] = l[i + 1] + d.y; l[i + 2] = l[i + 2] + d.z; l[i + 3] = l[i + 3] + d.w;
-            }
+          for (int i = 0; i < VE; i++) store_logit(e + i, l[i]);
+          if (wide_out) {
+            *reinterpret_cast<uint4*>(out - lead + u) = *reinterpret_cast<uint4*>(e);
           } else {
 #pragma unroll
-            for (int i = 0; i < VE; i++) l[i] = l[i] + (v + i >= 0 && v + i < p.vocab ? dense[v + i] : 0.f);
+            for (int i = 0; i < VE; i++) out[u - lead + i] = e[i];
           }
         }
-        if (table) {
-          const uint32_t bits = touched[(u - c0) >> 5] >> ((u - c0) & 31) & ((1u << VE) - 1);
-          if (bits) {
+        float top = l[0];  // fmaxf passes over a NaN
 #pragma unroll
-            for (int i = 0; i < VE; i++)
-              if (bits >> i & 1) l[i] = __uint_as_float(word[u - c0 + i]);
-          }
-        }
-        if (mask) {
-          const int at = max(v, 0) >> 5, sh = max(v, 0) & 31;
-          const uint32_t low = __ldg(mask + at);
-          const uint32_t high = sh + VE > 32 && (at + 1) * 32 < p.vocab ? __ldg(mask + at + 1) : 0u;
-          uint32_t allowed = __funnelshift_r(low, high, sh);
-          if (v < 0) allowed <<= -v;
-#pragma unroll
-          for (int i = 0; i < VE; i++)
-            if (!(allowed >> i & 1)) l[i] = -INFINITY;
-        }
-#pragma unroll
-        for (int i = 0; i < VE; i++) store_logit(e + i, l[i]);
-        if (inside) {
-          if (wide_out) {
-            *reinterpret_cast<uint4*>(out + v) = *reinterpret_cast<uint4*>(e);
-          } else if (out) {
-#pragma unroll
-            for (int i = 0; i < VE; i++) out[v + i] = e[i];
-          }
-          float top = l[0];  // fmaxf passes over a NaN
-#pragma unroll
-          for (int i = 1; i < VE; i++) top = fmaxf(top, l[i]);
-          if (top > bv) {
-            bv = top;
-#pragma unroll
-            for (int i = VE - 1; i >= 0; i--)
-              if (l[i] == top) bi = v + i;
-          }
-        } else {
-          for (int i = 0; i < VE; i++) {
-            if (v + i < 0 || v + i >= p.vocab) continue;
-            if (out) out[v + i] = e[i];
-            if (l[i] > bv) {
-              bv = l[i];
-              bi = v + i;
-            }
-          }
+        for (int i = 1; i < VE; i++) top = fmaxf(top, l[i]);
+        if (top > bv) {
+          bv = top;
+          bu = u;
+          piece = raw[j];
         }
       }
     }
+    if (bu >= 0) {
+      float l[VE];
+      values(piece, bu, l);
+      int i = VE - 1;
+#pragma unroll
+      for (int j = VE - 2; j >= 0; j--)
+        if (l[j] == bv) i = j;
+      best = max_key(best, pick_key(bv, bu - lead + i));
+    }
+    if (n) {
+      __syncthreads();  // the stream's stores are made
+      auto put = [&](int i, float l) {
+        const int v = v0 + list[i];
+        if (mask && !(mask[v >> 5] >> (v & 31) & 1)) l = -INFINITY;
+        if (out) store_logit(out + v, l);
+        best = max_key(best, pick_key(l, v));
+      };
+#pragma unroll
+      for (int j = 0; j < kSettle; j++)
+        if (t + j * threads < n) put(t + j * threads, settled(t + j * threads, mine[j], mine_dense[j]));
+      for (int i = t + kSettle * threads; i < n; i += threads) put(i, __uint_as_float(count[direct ? list[i] : i]));
+    }
   }
-  uint64_t best = pick_key(bv, bi);
   for (int o = 16; o; o >>= 1) best = max_key(best, __shfl_xor_sync(0xffffffffu, best, o));
   if ((t & 31) == 0) best_sm[t >> 5] = best;
   __syncthreads();
@@ -282,8 +345,10 @@ __global__ void __launch_bounds__(kMaxThreads) rules_kernel(const __grid_constan
     if (split > 1 && t == 0) dsmem_st64(dsmem_addr(&best_of[rank], 0), best);
   }
   if (split > 1) {
-    __syncwarp();
-    cluster_sync();  // the ranks' keys are in rank 0, and every rank has read the history
+    // Arrivals: the rank's key is in rank 0, and it has read the history. Only rank 0 waits.
+    cluster_arrive();
+    if (rank) return;
+    cluster_wait();
   }
   if (rank == 0 && t == 0) {
     for (int q = 0; q < (split > 1 ? split : 0); q++) best = max_key(best, best_of[q]);
@@ -300,25 +365,82 @@ __global__ void __launch_bounds__(kMaxThreads) rules_kernel(const __grid_constan
 
 }  // namespace
 
-// CTAs per row: one where it has at most 16,384 tokens to go through (a cluster costs more than its
-// share of the work saves), else enough for four per SM and for ranges of one chunk.
+namespace {
+template <auto Kernel>
+auto with_smem(size_t bytes) {
+  if (bytes > 46 * 1024) allow_smem<Kernel>(220 * 1024);
+  return Kernel;
+}
+
+// How many clusters of n CTAs run at once, asked once per device: clusters stay inside a group of
+// SMs, which leaves some SMs idle for most n.
+template <auto Kernel, int Threads, int PerSm>
+int64_t clusters_at_once(int n) {
+  static std::atomic<int> known[64][9];
+  int device = 0;
+  check_cuda(cudaGetDevice(&device), "cudaGetDevice");
+  std::atomic<int>* slot = device < 64 ? &known[device][n] : nullptr;
+  if (slot && slot->load(std::memory_order_relaxed)) return slot->load(std::memory_order_relaxed);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(n * PerSm * 148);
+  cfg.blockDim = dim3(Threads);
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = n;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int c = 0;
+  check_cuda(cudaOccupancyMaxActiveClusters(&c, Kernel, &cfg), "occupancy");
+  c = std::max(1, std::min(c, 148 * PerSm / n));
+  if (slot) slot->store(c, std::memory_order_relaxed);
+  return c;
+}
+
+// CTAs per row. One where it has at most 16,384 tokens to go through: a cluster costs more than its
+// share of the work saves. Up to 148 rows: the most that still run at once with an SM each (16
+// rows of 131,072 bf16 tokens without rules: 6 CTAs 4.3 us, 8 in two waves 7.4; 64 rows: 2 CTAs
+// 7.2, 8 CTAs 8.3). More rows: the number whose waves take the shortest, the lists and the
+// joining of a CTA's results counted like 12,000 tokens (192 rows of 131,072 bf16 tokens with all
+// rules: 5 CTAs 52 us, 2 CTAs 54, 8 CTAs 59, 1 CTA 85; 512 rows of 32,000: 1 CTA 11.3, 2 CTAs 14.3).
+template <class T>
+int rules_split(int64_t rows, int64_t span) {
+  if (span <= 16384) return 1;
+  int split = 1;
+  if (rows <= 148) {
+    for (int n = 2; n <= 8; n++)
+      if (rows <= clusters_at_once<rules_kernel<T, 512, 1>, 512, 1>(n)) split = n;
+    return split;
+  }
+  int64_t least = INT64_MAX;
+  for (int n = 1; n <= 8; n++) {
+    const int64_t at_once = clusters_at_once<rules_kernel<T, 256, 4>, 256, 4>(n);
+    const int64_t t = (rows + at_once - 1) / at_once * (span / n + 12000);
+    if (t < least) {
+      least = t;
+      split = n;
+    }
+  }
+  return split;
+}
+}  // namespace
+
 void launch_rules(const RulesParams& p, cudaStream_t s) {
   const int ve = p.bf16 ? 8 : 4;
   const int64_t span = (int64_t)p.vocab + ve - 1;  // with the lead of the worst row
-  int split = 1;
-  if (span > kMaxChunk)
-    while (split < 8 && (p.rows * split < 4 * 148 || span > (int64_t)split * kMaxChunk)) split *= 2;
+  const int entries = (p.rules.d_history ? p.rules.history_cap : 0) + (p.rules.d_bias_ids ? p.rules.bias_cap : 0);
+  const int split = p.bf16 ? rules_split<__nv_bfloat16>(p.rows, span) : rules_split<float>(p.rows, span);
   const int range = (int)((span + split - 1) / split + 31) / 32 * 32;
-  const int chunk = std::min(range, kMaxChunk);
-  // Two pieces per thread and more threads for a lone row, four and at most 256 threads for many.
-  const int most = p.rows * split <= 148 ? kMaxThreads : p.rows * split <= 2 * 148 ? 512 : 256;
+  const int chunk = std::min(range, entries > kLongLists ? kMaxChunkLong : kMaxChunk);
+  // Two pieces per thread; 512 threads where two CTAs per SM take all rows (256 rows of 4,001 f32
+  // tokens with all rules: 10 us, 13 with 256 threads).
+  const int64_t ctas = p.rows * split;
+  const int most = ctas <= 2 * 148 ? 512 : 256;
   const int threads = std::min(most, std::max(64, ((chunk + 2 * ve - 1) / (2 * ve) + 31) / 32 * 32));
-  auto kernel = p.bf16 ? rules_kernel<__nv_bfloat16> : rules_kernel<float>;
-  const size_t smem = p.rules.d_history || p.rules.d_bias_ids ? (size_t)chunk * 4 + chunk / 8 + kMaxTouched * 2 : 0;
-  if (smem > 46 * 1024) {
-    constexpr size_t kMost = kMaxChunk * 4 + kMaxChunk / 8 + kMaxTouched * 2;
-    p.bf16 ? allow_smem<rules_kernel<__nv_bfloat16>>(kMost) : allow_smem<rules_kernel<float>>(kMost);
-  }
+  const int direct = chunk <= kDirect;
+  const int slots = direct ? chunk : std::min(entries, chunk);
+  const size_t smem = entries ? (size_t)chunk / 4 + (size_t)slots * kSlotBytes : 0;
+  auto launch = [&](auto kernel) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.rows * split));
   cfg.blockDim = dim3(threads);
@@ -333,7 +455,18 @@ void launch_rules(const RulesParams& p, cudaStream_t s) {
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = split > 1 ? 2 : 1;
-  check_cuda(cudaLaunchKernelEx(&cfg, kernel, p, split, range, chunk), "rules launch");
+  check_cuda(cudaLaunchKernelEx(&cfg, kernel, p, split, range, chunk, slots, direct), "rules launch");
+  };
+  auto variant = [&](auto type) {
+    using T = decltype(type);
+    if (ctas <= 148)
+      launch(with_smem<rules_kernel<T, 512, 1>>(smem));
+    else if (ctas <= 2 * 148)
+      launch(with_smem<rules_kernel<T, 512, 2>>(smem));
+    else
+      launch(with_smem<rules_kernel<T, 256, 4>>(smem));
+  };
+  p.bf16 ? variant(__nv_bfloat16()) : variant(float());
 }
 
 }  // namespace svl

@@ -224,3 +224,30 @@ def test_only_tokens_or_only_logits(svl_lib):
     ok(lib().svl_logits_rules_device(0, 6, 1000, 0, l.data_ptr(), 1000, None, out.data_ptr(), 1000, None, None))
     torch.cuda.synchronize()
     assert torch.equal(out, l) and torch.equal(tok.long(), l.argmax(1))
+
+
+@pytest.mark.parametrize("rows,vocab,history,biased,dtype", [
+    (1, 140000, 9000, 300, "f32"),     # two chunks per CTA, lists too long for a slot each in one
+    (1, 1100001, 700, 5, "bf16"),      # chunks without room for a whole eighth
+    (150, 20001, 60, 9, "bf16"),       # more rows than SMs
+    (300, 16390, 2100, 0, "f32"),      # history entries past the first in flight
+    (33, 131072, 40, 8, "bf16")])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_splits_and_chunks(svl_lib, rows, vocab, history, biased, dtype, in_place):
+    g, r = make(rows, vocab, rows + vocab, history=history, biased=biased, dense=True, masks=2)
+    check((4 * g.standard_normal((rows, vocab))).astype(F), r, dtype, offset=rows % 8, in_place=in_place)
+
+
+def test_edges_of_rows(svl_lib):
+    """The best token at each end of rows that start off their alignment, touched or not, and no
+    other token left in between."""
+    for vocab in (1, 2, 3, 4, 5, 7, 8, 9, 15, 16, 17, 33):
+        for offset in range(8):
+            for at in {0, vocab - 1, vocab // 2}:
+                logits = np.zeros((3, vocab), F)
+                logits[:, at] = 5
+                r = {"history": np.full((3, 4), at, np.int32), "lengths": np.array([0, 1, 4], np.int32),
+                     "frequency": np.full(3, 2, F), "presence": np.zeros(3, F), "repetition": np.ones(3, F)}
+                for dtype in ("f32", "bf16"):
+                    check(logits, r, dtype, offset=offset)
+                    check(logits, {}, dtype, offset=offset, in_place=True)
