@@ -15,6 +15,7 @@
 //
 // No load here uses cluster multicast.
 #include <algorithm>
+#include <type_traits>
 #include <cuda_bf16.h>
 
 #include "common.cuh"
@@ -342,12 +343,12 @@ struct RowStore {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(pad + place(lane, j)), "r"(a), "r"(b), "r"(c), "r"(d)
                  : "memory");
   }
-  // The chunk that starts at column n0 (those of its columns that exist).
+  // The chunk that starts at column n0 (those of its first `width` columns that exist).
   template <class T>
-  __device__ __forceinline__ void out(int n0) const {
+  __device__ __forceinline__ void out(int n0, int width = 32 / sizeof(T)) const {
     constexpr int kPer = 16 / sizeof(T), kCols = 32 / sizeof(T);
     __syncwarp();
-    const int cols = min(kCols, p.m.n - n0);
+    const int cols = min(width, p.m.n - n0);
     T* base = static_cast<T*>(p.out) + r0 * p.out_stride + n0;
     if (aligned && cols == kCols) {
       const int j = lane & 1;
@@ -362,21 +363,22 @@ struct RowStore {
         if (r0 + row < p.rows) *reinterpret_cast<uint4*>(base + row * p.out_stride + j * kPer) = v;
       }
     } else {
-      const int rows = (int)min((int64_t)32, p.rows - r0);
-      for (int i = lane; i < rows * kCols; i += 32) {
-        const int row = i / kCols, c = i % kCols;
-        if (c >= cols) continue;
-        const uint32_t from = pad + place(row, c / kPer) + c % kPer * sizeof(T);
-        if constexpr (sizeof(T) == 4) {
-          uint32_t v;
-          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(from) : "memory");
-          reinterpret_cast<uint32_t*>(base)[row * p.out_stride + c] = v;
-        } else {
-          uint16_t v;
-          asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(from) : "memory");
-          reinterpret_cast<uint16_t*>(base)[row * p.out_stride + c] = v;
-        }
+      // One column per lane; four (two) rows per instruction, the shared-memory reads of all first.
+      using U = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
+      const int c = lane % kCols, row0 = lane / kCols;
+      U v[kCols];
+#pragma unroll
+      for (int i = 0; i < kCols; i++) {
+        const uint32_t from = pad + place(row0 + i * (32 / kCols), c / kPer) + c % kPer * sizeof(T);
+        if constexpr (sizeof(T) == 4)
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v[i]) : "r"(from) : "memory");
+        else
+          asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v[i]) : "r"(from) : "memory");
       }
+      U* to = reinterpret_cast<U*>(base) + row0 * p.out_stride + c;
+#pragma unroll
+      for (int i = 0; i < kCols; i++, to += 32 / kCols * p.out_stride)
+        if (c < cols && r0 + row0 + i * (32 / kCols) < p.rows) *to = v[i];
     }
     __syncwarp();
   }
@@ -642,29 +644,27 @@ __global__ void __launch_bounds__(Wide::kThreads, 1) f8_wide_kernel(const __grid
             y[0] += u.x; y[1] += u.y; y[2] += u.z; y[3] += u.w;
             y[4] += v.x; y[5] += v.y; y[6] += v.z; y[7] += v.w;
           }
-          if (r >= p.rows) continue;
-          const bool whole = rs.aligned && n + 8 <= p.m.n;
           if (p.m.bias) {
 #pragma unroll
             for (int e = 0; e < 8; e++) y[e] = y[e] + bias_at(n + e);
           }
-          if (bf16) {
-            __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + r * p.out_stride + n;
-            if (whole)
+          if (rs.aligned && n + 8 <= p.m.n) {
+            if (r >= p.rows) continue;
+            if (bf16) {
+              __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + r * p.out_stride + n;
               *reinterpret_cast<uint4*>(o) = make_uint4(bf16_pair(y[0], y[1]), bf16_pair(y[2], y[3]), bf16_pair(y[4], y[5]), bf16_pair(y[6], y[7]));
-            else
-#pragma unroll
-              for (int e = 0; e < 8; e++)
-                if (n + e < p.m.n) o[e] = __float2bfloat16_rn(y[e]);
-          } else {
-            float* o = static_cast<float*>(p.out) + r * p.out_stride + n;
-            if (whole) {
+            } else {
+              float* o = static_cast<float*>(p.out) + r * p.out_stride + n;
               reinterpret_cast<float4*>(o)[0] = make_float4(y[0], y[1], y[2], y[3]);
               reinterpret_cast<float4*>(o)[1] = make_float4(y[4], y[5], y[6], y[7]);
-            } else
-#pragma unroll
-              for (int e = 0; e < 8; e++)
-                if (n + e < p.m.n) o[e] = y[e];
+            }
+          } else if (bf16) {
+            rs.piece(0, bf16_pair(y[0], y[1]), bf16_pair(y[2], y[3]), bf16_pair(y[4], y[5]), bf16_pair(y[6], y[7]));
+            rs.out<__nv_bfloat16>(n, 8);
+          } else {
+            rs.piece(0, __float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
+            rs.piece(1, __float_as_uint(y[4]), __float_as_uint(y[5]), __float_as_uint(y[6]), __float_as_uint(y[7]));
+            rs.out<float>(n);
           }
         }
       }
@@ -946,15 +946,13 @@ void launch_thin(F8Args a, cudaStream_t s) {
 
 // 128 x 128 tiles. The exchange of a split tile costs about as much as 9 blocks, so it is split only
 // where it saves more (256 x 2048 x 5632, 32 tiles: 16.5 us alone, 12.5 with 2, 10.4 with 4; 256 x
-// 6144 x 2048, 96 tiles: 9.3 alone, 16.9 with 2), and where outputs can be stored in 16-byte pieces.
+// 6144 x 2048, 96 tiles: 9.3 alone, 16.9 with 2).
 void launch_wide(F8Args a, cudaStream_t s) {
   const CUtensorMap map = plan(a, Wide::kTN, kF8Block);
   const int tiles = a.ntiles * a.rtiles;
-  const bool aligned = reinterpret_cast<uintptr_t>(a.p.out) % 16 == 0 && a.p.out_stride % (a.p.out_bf16 ? 8 : 4) == 0;
   a.split = 1;
-  if (aligned)
-    for (int S : {2, 4})
-      if (tiles * S <= kSms && a.kblocks * (S - 1) > 9 * S) a.split = S;
+  for (int S : {2, 4})
+    if (tiles * S <= kSms && a.kblocks * (S - 1) > 9 * S) a.split = S;
   const int grid = a.split > 1 ? tiles * a.split : std::min(tiles, kSms);
   launch<f8_wide_kernel>(dim3(grid), Wide::kThreads, Wide::kSmem, a.split, map, a, s);
 }

@@ -218,6 +218,23 @@ def test_linear_padded(svl_lib, rows):
     assert torch.equal(got, lin(d["q"], d["s"]))
 
 
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,n,k", [(100, 131, 8200), (128, 4001, 2500), (129, 257, 2600), (65, 135, 6000), (130, 8, 5000)])
+def test_linear_odd_outputs(svl_lib, rows, n, k, out):
+    """Outputs of an odd width at an odd offset, also where CTAs share a tile; nothing outside is written."""
+    import torch
+
+    import svl
+    d = quantised(rows, k, n, rows + n, bias=True)
+    lin = svl.F8Linear(d["w"], d["ws"], d["b"])
+    big = torch.full((rows + 2, n + 6), -1.0, device="cuda", dtype=torch_dtype(out))
+    got = lin(d["q"], d["s"], out=big[1:rows + 1, 5:5 + n])
+    check_linear(got, d, out)
+    outside = big.clone()
+    outside[1:rows + 1, 5:5 + n] = -1.0
+    assert torch.all(outside == -1.0)
+
+
 def test_linear_quantise(svl_lib):
     """F8Linear.quantise's weights are within half an e4m3 step of the f32 ones."""
     import torch
