@@ -11,6 +11,7 @@
 #include "common.cuh"
 #include "engine.h"
 #include "rules.cuh"
+#include "sm100.cuh"
 
 namespace svl {
 namespace {
@@ -33,6 +34,8 @@ __global__ void qkv_kernel(const QkvParams p) {
   const int pairs = (p.q_dim + 2 * p.kv_dim) / 2, half = p.head_dim / 2;
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
   const int b = blockIdx.y;
+  pdl_launch();
+  pdl_wait();
   if (i >= pairs) return;
   const float2 v = reinterpret_cast<const float2*>(p.y + (int64_t)b * 2 * pairs)[i];
   const int row = 2 * i;
@@ -74,6 +77,8 @@ template <int FFN>
 __global__ void __launch_bounds__(256) act_f8_kernel(const ActParams p) {
   const int b = blockIdx.y, lane = threadIdx.x & 31;
   const int block = blockIdx.x * 8 + (threadIdx.x >> 5);
+  pdl_launch();
+  pdl_wait();
   if (block * kF8Block >= p.f) return;
   const float* y = p.y + (int64_t)b * p.y_stride;
   const int c = block * kF8Block + lane * 4;
@@ -99,6 +104,21 @@ __global__ void __launch_bounds__(256) act_f8_kernel(const ActParams p) {
   for (int j = 0; j < 4; j++)
     if (c + j < p.f) q[j] = to_e4m3(z[j] * inv);
   if (lane == 0) p.scales[(int64_t)block * p.scale_stride + b] = __fdiv_rn(top, kF8Max);
+}
+
+// A launch whose setup runs beside the end of the kernel before.
+template <class P>
+void launch_early(void (*kernel)(const P), dim3 grid, const P& p, cudaStream_t st, const char* what) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  check_cuda(cudaLaunchKernelEx(&cfg, kernel, p), what);
 }
 
 int64_t padded(int k) { return (k + 15) / 16 * 16; }
@@ -172,8 +192,7 @@ void enqueue_layers_f8(Model& m, State& s, int b0, int nb, cudaStream_t st, bool
       product(s, L.in_proj, nb, y, st);
       const GemvParams& g = lp.in_proj;
       const QkvParams k{y, rope_cs, pos, nb, qd, kvd, hd, g.ring_cap, g.windowed, g.kv_bf16, g.out, g.k_ring, g.v_ring, g.ring_stream_stride};
-      qkv_kernel<<<dim3(((qd + 2 * kvd) / 2 + 255) / 256, nb), 256, 0, st>>>(k);
-      check_cuda(cudaGetLastError(), "RoPE launch");
+      launch_early(qkv_kernel, dim3(((qd + 2 * kvd) / 2 + 255) / 256, nb), k, st, "RoPE launch");
     }
     if (do_attn) launch_attention_decode(lp.attn, st);
     if (!do_lin) continue;
@@ -184,13 +203,10 @@ void enqueue_layers_f8(Model& m, State& s, int b0, int nb, cudaStream_t st, bool
     const int f = c.ffn_hidden;
     const ActParams a{y, L.ff1.n, f, s.f8_q.as<uint8_t>(), padded(f), s.f8_s.as<float>(), s.max_batch};
     const dim3 grid((f + 8 * kF8Block - 1) / (8 * kF8Block), nb);
-    if (c.ffn_kind == SVL_FFN_GATED_SILU)
-      act_f8_kernel<SVL_FFN_GATED_SILU><<<grid, 256, 0, st>>>(a);
-    else if (c.ffn_kind == SVL_FFN_PLAIN_GELU_TANH)
-      act_f8_kernel<SVL_FFN_PLAIN_GELU_TANH><<<grid, 256, 0, st>>>(a);
-    else
-      act_f8_kernel<SVL_FFN_PLAIN_GELU_ERF><<<grid, 256, 0, st>>>(a);
-    check_cuda(cudaGetLastError(), "activation launch");
+    const auto act = c.ffn_kind == SVL_FFN_GATED_SILU      ? act_f8_kernel<SVL_FFN_GATED_SILU>
+                     : c.ffn_kind == SVL_FFN_PLAIN_GELU_TANH ? act_f8_kernel<SVL_FFN_PLAIN_GELU_TANH>
+                                                             : act_f8_kernel<SVL_FFN_PLAIN_GELU_ERF>;
+    launch_early(act, grid, a, st, "activation launch");
     product(s, L.ff2, nb, delta, st);
   }
 }
