@@ -476,8 +476,12 @@ SVL_API void svl_f8_linear_destroy(svl_f8_linear* linear) {
   if (!linear) return;
   entry([&] {
     OnDevice on(linear->device);
-    cudaDeviceSynchronize();
+    // cudaFree waits for the device. A collector may come here while some thread captures a graph,
+    // which a call that may wait would end, but for this mode.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
     delete linear;
+    cudaThreadExchangeStreamCaptureMode(&mode);
   });
 }
 

@@ -76,10 +76,7 @@ int32_t dtype_of(const char* name, at::ScalarType t) {
   refuse(std::string(name) + " must be float32 or bfloat16");
 }
 
-void* stream_of(PyObject* given, c10::Device dev) {
-  if (given != Py_None) return PyLong_AsVoidPtr(given);
-  return c10::cuda::getCurrentCUDAStream(dev.index()).stream();
-}
+void* current_stream(c10::Device dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
 
 at::Tensor empty(at::IntArrayRef size, at::ScalarType type, c10::Device dev) {
   return at::detail::empty_cuda(size, type, dev, std::nullopt);
@@ -103,10 +100,10 @@ bool count(Py_ssize_t got, Py_ssize_t want) {
   return false;
 }
 
-// x, residual, norm kind, weight, bias, eps, out_sum, stream -> (q, scales, h)
+// x, residual, norm kind, weight, bias, eps, out_sum -> (q, scales, h)
 PyObject* add_norm_f8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (!count(n, 8)) return nullptr;
+  if (!count(n, 7)) return nullptr;
   const at::Tensor& x = *tensor("x", a[0]);
   check_rows("x", x);
   const int64_t rows = x.size(0), k = x.size(1), ld = (k + 15) / 16 * 16;
@@ -131,7 +128,7 @@ PyObject* add_norm_f8(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                   row_stride(x), residual ? residual->data_ptr() : nullptr,
                                   residual ? row_stride(*residual) : 0, (int32_t)kind, w, b, (float)eps,
                                   keep ? h.data_ptr() : nullptr, row_stride(h), static_cast<uint8_t*>(q.data_ptr()), ld,
-                                  static_cast<float*>(scales.data_ptr()), rows, stream_of(a[7], dev));
+                                  static_cast<float*>(scales.data_ptr()), rows, current_stream(dev));
   if (!done(s)) return nullptr;
   PyObject* out = PyTuple_New(3);
   if (!out) return nullptr;
@@ -148,10 +145,10 @@ PyObject* add_norm_f8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// handle, n, k, device index, q, scales, out dtype, out, stream -> out
+// handle, n, k, device index, q, scales, out dtype, out -> out
 PyObject* f8_linear(PyObject*, PyObject* const* a, Py_ssize_t cnt) {
   HANDLE_TH_ERRORS
-  if (!count(cnt, 9)) return nullptr;
+  if (!count(cnt, 8)) return nullptr;
   void* handle = PyLong_AsVoidPtr(a[0]);
   const long n = PyLong_AsLong(a[1]), k = PyLong_AsLong(a[2]), index = PyLong_AsLong(a[3]);
   if (PyErr_Occurred()) return nullptr;
@@ -171,7 +168,7 @@ PyObject* f8_linear(PyObject*, PyObject* const* a, Py_ssize_t cnt) {
   const int64_t ld = rows > 1 ? q.stride(0) : (k + 15) / 16 * 16;
   const svl_status s = g_linear(static_cast<svl_f8_linear*>(handle), rows, static_cast<const uint8_t*>(q.data_ptr()), ld,
                                 static_cast<const float*>(scales.data_ptr()), row_stride(scales), dtype, out.data_ptr(),
-                                row_stride(out), stream_of(a[8], dev));
+                                row_stride(out), current_stream(dev));
   if (!done(s)) return nullptr;
   if (given) {
     Py_INCREF(a[7]);
@@ -182,10 +179,10 @@ PyObject* f8_linear(PyObject*, PyObject* const* a, Py_ssize_t cnt) {
 }
 
 // logits, history, lengths, repetition, frequency, presence, dense_bias, bias_ids, bias_values,
-// masks, mask_rows, first_penalised, append, out, stream -> (logits, tokens)
+// masks, mask_rows, first_penalised, append, out -> (logits, tokens)
 PyObject* logits_rules(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (!count(n, 15)) return nullptr;
+  if (!count(n, 14)) return nullptr;
   const at::Tensor& logits = *tensor("logits", a[0]);
   check_rows("logits", logits);
   const int64_t rows = logits.size(0), vocab = logits.size(1);
@@ -246,7 +243,7 @@ PyObject* logits_rules(PyObject*, PyObject* const* a, Py_ssize_t n) {
   at::Tensor tokens = empty({rows}, at::kInt, dev);
   const svl_status s = g_rules(dev.index(), rows, (int32_t)std::min<int64_t>(vocab, INT32_MAX), dtype, logits.data_ptr(),
                                row_stride(logits), &r, out.data_ptr(), row_stride(out),
-                               static_cast<int32_t*>(tokens.data_ptr()), stream_of(a[14], dev));
+                               static_cast<int32_t*>(tokens.data_ptr()), current_stream(dev));
   if (!done(s)) return nullptr;
   PyObject* both = PyTuple_New(2);
   if (!both) return nullptr;

@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import ctypes
 
-import torch  # noqa: F401  (the binding's symbols)
+import torch  # the binding's symbols too
 
 from . import _lib
 
@@ -22,6 +22,9 @@ ops.bind(_address("svl_add_norm_f8_device"), _address("svl_f8_linear_device"), _
          _address("svl_last_error"), _lib.SvlError)
 
 
-def raw_stream(stream):
-    """The handle of a torch stream; None for the current one."""
-    return None if stream is None else stream.cuda_stream
+def on(stream, device):
+    """The context in which a call runs and allocates on `stream`, a stream of the tensors' device.
+    (Outputs that belonged to another stream could be given out again while `stream` still writes.)"""
+    if stream.device != device:
+        raise ValueError(f"stream must be one of {device}: got one of {stream.device}")
+    return torch.cuda.stream(stream)

@@ -12,7 +12,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._ops import ops, raw_stream
+from ._ops import on, ops
 from .model import tensor_views
 
 BLOCK = 128
@@ -26,16 +26,20 @@ def add_norm_f8(x, residual=None, norm: str | None = "rms", weight=None, bias=No
     x and residual: CUDA [rows, k], float32 or bfloat16; weight and bias: float32 [k] or None.
     Returns (q, scales, h): q float8_e4m3fn [rows, k] (rows 16-byte aligned), scales float32
     [ceil(k / 128), rows], and the sum h in x's dtype: out_sum if given (it may be x or residual),
-    a new tensor with a residual, x itself without."""
+    a new tensor with a residual, x itself without. out_sum must not overlap x or residual otherwise."""
+    if stream is not None:
+        with on(stream, x.device):
+            return add_norm_f8(x, residual, norm, weight, bias, eps, out_sum)
     kind = _NORMS.get(norm, 2)  # 2: refused by name below the binding
-    return ops.add_norm_f8(x, residual, kind, weight, bias, eps, out_sum, raw_stream(stream))
+    return ops.add_norm_f8(x, residual, kind, weight, bias, eps, out_sum)
 
 
 class F8Linear:
     """An e4m3 matrix [n][k] with f32 scales per 128 x 128 block, and an optional bias.
 
     weight: float8_e4m3fn CUDA [n, k], scales: float32 CUDA [ceil(n / 128), ceil(k / 128)], bias:
-    float32 CUDA [n] or None; all are copied. F8Linear.quantise() makes one from f32 weights."""
+    float32 CUDA [n] or None; all are copied. F8Linear.quantise() makes one from f32 weights. It has to
+    outlive the CUDA graphs that captured its products."""
 
     handle = None
 
@@ -82,7 +86,10 @@ class F8Linear:
         counts then)."""
         if self.handle is None:
             raise ValueError("the F8Linear is closed")
-        return ops.f8_linear(self.handle, self.n, self.k, self.device, q, scales, out_dtype, out, raw_stream(stream))
+        if stream is not None:
+            with on(stream, torch.device("cuda", self.device)):
+                return self(q, scales, out_dtype, out)
+        return ops.f8_linear(self.handle, self.n, self.k, self.device, q, scales, out_dtype, out)
 
     def check(self):
         """Waits for the device; raises if a bounded device-side wait of a product ran out."""

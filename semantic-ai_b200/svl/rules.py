@@ -4,7 +4,7 @@ from __future__ import annotations
 
 import ctypes
 
-from ._ops import ops, raw_stream
+from ._ops import on, ops
 
 
 class CLogitsRules(ctypes.Structure):
@@ -31,6 +31,11 @@ def logits_rules(logits, history=None, lengths=None, repetition=None, frequency=
     Ids below first_penalised are never penalised; append records the picked tokens.
     dense_bias float32 [vocab]; bias_ids int32 and bias_values float32 [rows, entries] (ids
     outside the vocabulary are pads). masks int32 [n, words of 32 tokens], a set bit allows its
-    token; mask_rows int32 [rows] chooses a row's mask (-1: none; without it, row r takes mask r)."""
+    token; mask_rows int32 [rows] chooses a row's mask (-1: none; without it, row r takes mask r).
+    `out` must not overlap logits unless it is logits."""
+    if stream is not None:
+        with on(stream, logits.device):
+            return logits_rules(logits, history, lengths, repetition, frequency, presence, dense_bias, bias_ids,
+                                bias_values, masks, mask_rows, first_penalised, append, out)
     return ops.logits_rules(logits, history, lengths, repetition, frequency, presence, dense_bias, bias_ids, bias_values,
-                            masks, mask_rows, first_penalised, append, out, raw_stream(stream))
+                            masks, mask_rows, first_penalised, append, out)

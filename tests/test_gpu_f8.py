@@ -323,3 +323,52 @@ def test_streams_and_graphs(svl_lib):
     torch.cuda.synchronize()
     assert torch.equal(y, other) and torch.equal(h, other_h) and torch.equal(y2, other)
     lin.check()
+
+
+def test_outputs_belong_to_their_stream(svl_lib):
+    """Outputs of a call on another stream are not given out again while that stream has yet to write them."""
+    import torch
+
+    import svl
+    side = torch.cuda.Stream()
+    x = torch.randn(64, 4096, device="cuda")
+    lin = svl.F8Linear.quantise(np.ones((256, 4096), np.float32))
+    q, s, _ = svl.add_norm_f8(x)
+    lg = lin(q, s)
+    for call in (lambda: svl.add_norm_f8(x, x, stream=side), lambda: lin(q, s, stream=side), lambda: svl.logits_rules(lg, stream=side)):
+        for warm in (True, False):  # loading a kernel for the first time waits for the device
+            torch.cuda.synchronize()
+            with torch.cuda.stream(side):
+                torch.cuda._sleep(100_000_000)
+            got = call()
+            sizes = [(t.shape, t.dtype) for t in (got if isinstance(got, tuple) else (got,)) if t is not x]
+            del got
+            taken = [torch.full(shape, 7.0, device="cuda").to(dtype) for shape, dtype in sizes for _ in range(2)]
+            torch.cuda.current_stream().synchronize()
+            waiting = not side.query()
+            side.synchronize()
+            assert all(torch.all(t.float() == 7.0) for t in taken)
+        assert waiting, "the side stream had ended before the memory was taken"
+    side.synchronize()
+    if torch.cuda.device_count() > 1:
+        with pytest.raises(ValueError, match="stream must"):
+            svl.add_norm_f8(x, stream=torch.cuda.Stream(1))
+
+
+def test_linear_closed_during_capture(svl_lib):
+    """An F8Linear that goes away while a graph is captured (as the collector may decide) leaves the capture alone."""
+    import torch
+
+    import svl
+    x = torch.randn(3, 256, device="cuda")
+    lin, other = (svl.F8Linear.quantise(np.eye(256, dtype=np.float32)) for _ in range(2))
+    q, s, _ = svl.add_norm_f8(x, norm=None)
+    want = lin(q, s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q2, s2, _ = svl.add_norm_f8(x, norm=None)
+        other.close()
+        got = lin(q2, s2)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
