@@ -224,7 +224,7 @@ __global__ void f8_pack_kernel(const uint8_t* src, int64_t stride, int n, int k,
 // One CTA per 128 x 128 block: its largest magnitude, its scale, its e4m3 values.
 __global__ void __launch_bounds__(256) f8_quantise_kernel(const float* src, int n, int k, uint8_t* dst, float* scales) {
   __shared__ float red[8];
-  const int kb = blockIdx.x, tile = blockIdx.y, kblocks = gridDim.x;
+  const int tile = blockIdx.x, kb = blockIdx.y, kblocks = gridDim.y;
   auto value = [&](int i) -> float {
     const int r = tile * kF8Block + i / kF8Block, c = kb * kF8Block + i % kF8Block;
     if (r >= n || c >= k) return 0.f;
@@ -327,7 +327,7 @@ void launch_f8_pack(const uint8_t* src, int64_t stride, int n, int k, uint8_t* d
 }
 
 void launch_f8_quantise(const float* src, int n, int k, uint8_t* dst, float* scales, cudaStream_t s) {
-  const dim3 grid((k + kF8Block - 1) / kF8Block, (n + kF8Block - 1) / kF8Block);
+  const dim3 grid((n + kF8Block - 1) / kF8Block, (k + kF8Block - 1) / kF8Block);  // up to 2^17 x 2^13
   f8_quantise_kernel<<<grid, 256, 0, s>>>(src, n, k, dst, scales);
   check_cuda(cudaGetLastError(), "quantise launch");
 }

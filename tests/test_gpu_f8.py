@@ -257,6 +257,22 @@ def test_linear_quantise(svl_lib):
             assert np.all(np.abs(got[blk] - w[blk]) <= half), (i, j)
 
 
+def test_linear_many_outputs(svl_lib):
+    """More than 65,535 tiles of matrix rows."""
+    import torch
+
+    import svl
+    n = 65536 * 128 + 5
+    w = np.ones((n, 1), np.float32)
+    w[::2] = -0.5
+    lin = svl.F8Linear.quantise(w)
+    q, s, _ = svl.add_norm_f8(torch.tensor([[3.0], [-8.0]], device="cuda"), norm=None)
+    got = lin(q, s)
+    # The row's and the matrix's scales round once each, the products twice.
+    want = torch.tensor([[3.0], [-8.0]], device="cuda") * torch.from_numpy(w).cuda().t()
+    assert torch.all((got - want).abs() <= want.abs() * 4 * 2.0 ** -24)
+
+
 def test_linear_refuses(svl_lib):
     import torch
 
