@@ -325,8 +325,9 @@ __global__ void __launch_bounds__(Thin<BN>::kThreads, 2)
   if (warp == C::kEpiWarps + 1) tmem_free(tmem, C::kCols);
 }
 
-// Stores chunks of 32 bytes per row (8 f32 or 16 bf16 columns) for the 32 rows a warp's lanes hold.
-// Through shared memory (the two 16-byte pieces swapped in every other group of four rows, so that
+// Stores chunks of 32 bytes per row (8 f32 or 16 bf16 columns) for the 32 rows a warp's lanes hold,
+// where a lane cannot store whole sectors itself (rows that start off 32 bytes, a tile's cut last
+// columns). Through shared memory (the two 16-byte pieces swapped in every other group of four rows, so that
 // neither side has bank conflicts): a lane's own row would make every store touch half a sector
 // of 32 lines; this way a store instruction covers whole sectors of 16 rows.
 struct RowStore {
@@ -336,6 +337,7 @@ struct RowStore {
   int lane;
   int64_t r0;     // the row of lane 0
   bool aligned;   // rows start on 16 bytes
+  bool sectors;   // rows start on 32 bytes
 
   static __device__ __forceinline__ uint32_t place(int row, int j) { return row * 32 + ((j ^ ((row >> 2) & 1)) << 4); }
   // Piece j of this lane's row: 4 f32 or 8 bf16 values.
@@ -389,7 +391,16 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// A thread's sums of columns [n0, n0 + N) of its row, plus the bias, stored by its warp.
+// 32 bytes (a sector), 32-byte aligned.
+__device__ __forceinline__ void store_sector(void* to, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+// A thread's sums of columns [n0, n0 + N) of its row, plus the bias. Each lane stores the sectors of
+// its own row where they are whole (1030 x 11264 x 2048 bf16: 36.4 us; 38.5 with every chunk through
+// shared memory), else its warp does together.
 template <int N>
 __device__ __forceinline__ void store_sums(const RowStore& rs, uint64_t (&acc)[N / 2], int n0, bool bf16) {
   const F8GemmParams& p = rs.p;
@@ -398,6 +409,33 @@ __device__ __forceinline__ void store_sums(const RowStore& rs, uint64_t (&acc)[N
     for (int c = 0; c < N; c += 2)
       acc[c / 2] = pair_of(pair_lo(acc[c / 2]) + (n0 + c < p.m.n ? p.m.bias[n0 + c] : 0.f),
                            pair_hi(acc[c / 2]) + (n0 + c + 1 < p.m.n ? p.m.bias[n0 + c + 1] : 0.f));
+  }
+  if (rs.sectors && n0 + N <= p.m.n) {
+    const int64_t r = rs.r0 + rs.lane;
+    if (r >= p.rows) return;
+    if (bf16) {
+      __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.out) + r * p.out_stride + n0;
+#pragma unroll
+      for (int c = 0; c < N; c += 16) {
+        uint32_t v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = bf16_pair(pair_lo(acc[c / 2 + e]), pair_hi(acc[c / 2 + e]));
+        store_sector(to + c, v);
+      }
+    } else {
+      float* to = static_cast<float*>(p.out) + r * p.out_stride + n0;
+#pragma unroll
+      for (int c = 0; c < N; c += 8) {
+        uint32_t v[8];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          v[2 * e] = (uint32_t)acc[c / 2 + e];
+          v[2 * e + 1] = (uint32_t)(acc[c / 2 + e] >> 32);
+        }
+        store_sector(to + c, v);
+      }
+    }
+    return;
   }
   if (bf16) {
 #pragma unroll
@@ -556,7 +594,8 @@ __global__ void __launch_bounds__(Wide::kThreads, 1) f8_wide_kernel(const __grid
     const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * C::kCpt;
     const bool bf16 = p.out_bf16;
     RowStore rs{p, smem_addr(smem + C::kRing) + warp * RowStore::kPad, lane, 0,
-                reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.out_stride % (bf16 ? 8 : 4) == 0};
+                reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.out_stride % (bf16 ? 8 : 4) == 0,
+                reinterpret_cast<uintptr_t>(p.out) % 32 == 0 && p.out_stride % (bf16 ? 16 : 8) == 0};
     auto bias_at = [&](int n) { return p.m.bias && n < p.m.n ? p.m.bias[n] : 0.f; };
     int buf = 0;
     uint32_t parity = 0;
@@ -871,7 +910,8 @@ __global__ void __launch_bounds__(Big::kThreads, 1) f8_big_kernel(const __grid_c
       const bool bf16 = p.out_bf16;
       const RowStore rs{p, smem_addr(smem + C::kRing) + warp * RowStore::kPad, lane,
                         (int64_t)(tile / a.ntiles) * kF8Block + (warp & 3) * 32,
-                        reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.out_stride % (bf16 ? 8 : 4) == 0};
+                        reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.out_stride % (bf16 ? 8 : 4) == 0,
+                        reinterpret_cast<uintptr_t>(p.out) % 32 == 0 && p.out_stride % (bf16 ? 16 : 8) == 0};
       store_sums<C::kCpt>(rs, acc, n0, bf16);
     }
   }
