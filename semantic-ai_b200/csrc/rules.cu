@@ -17,6 +17,35 @@ __device__ __forceinline__ float load_logit(const __nv_bfloat16* p) { return __b
 __device__ __forceinline__ void store_logit(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_logit(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
+// 16 bytes of logits.
+template <class T>
+__device__ __forceinline__ void unpack_logits(const uint4& v, float* l) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if constexpr (sizeof(T) == 4) {
+      l[i] = __uint_as_float(w[i]);
+    } else {
+      l[2 * i] = __uint_as_float(w[i] << 16);
+      l[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+}
+template <class T>
+__device__ __forceinline__ uint4 pack_logits(const float* l) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if constexpr (sizeof(T) == 4) {
+      w[i] = __float_as_uint(l[i]);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(l[2 * i], l[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // 16 bytes that are read once.
 __device__ __forceinline__ uint4 load_once(const void* p) {
   uint4 v;
@@ -241,11 +270,8 @@ __global__ void __launch_bounds__(Threads, PerSm) rules_kernel(const __grid_cons
     }
     // A piece's values; those of touched and forbidden tokens are -infinity.
     auto values = [&](const uint4& piece, int u, float* l) {
-      T e[VE];
-      *reinterpret_cast<uint4*>(e) = piece;
       const int v = u - lead;
-#pragma unroll
-      for (int i = 0; i < VE; i++) l[i] = load_logit(e + i);
+      unpack_logits<T>(piece, l);
       if (dense) {
         if (wide_bias) {
 #pragma unroll
@@ -292,12 +318,11 @@ __global__ void __launch_bounds__(Threads, PerSm) rules_kernel(const __grid_cons
         float l[VE];
         values(raw[j], u, l);
         if (out) {
-          T e[VE];
-#pragma unroll
-          for (int i = 0; i < VE; i++) store_logit(e + i, l[i]);
+          const uint4 packed = pack_logits<T>(l);
           if (wide_out) {
-            *reinterpret_cast<uint4*>(out - lead + u) = *reinterpret_cast<uint4*>(e);
+            *reinterpret_cast<uint4*>(out - lead + u) = packed;
           } else {
+            const T* e = reinterpret_cast<const T*>(&packed);
 #pragma unroll
             for (int i = 0; i < VE; i++) out[u - lead + i] = e[i];
           }
