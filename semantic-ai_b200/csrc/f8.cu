@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <memory>
 #include <string>
+#include <type_traits>
 
 #include "common.cuh"
 #include "entry.h"
@@ -67,6 +68,100 @@ __device__ __forceinline__ Raw<T, V> pack(const float (&v)[V]) {
   return r;
 }
 
+// Rows that start anywhere. A thread's V values are read in the aligned 16-byte pieces that hold at
+// least one of them (one more than V values take), as they come; `shifted` then cuts the values
+// out. (Value by value, every load of a warp would touch a sector per lane: 16,384
+// x 2,561 with a residual bf16 took 254 us, 120 this way.)
+template <class T, int V>
+struct RawOdd {
+  uint4 v[V * sizeof(T) / 16 + 1];
+};
+template <class T, int V>
+__device__ __forceinline__ RawOdd<T, V> load_odd(const T* p, int have) {
+  constexpr int N = V * sizeof(T) / 16;
+  const int off = (int)(reinterpret_cast<uintptr_t>(p) & 15);
+  const uint4* base = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) - off);
+  RawOdd<T, V> r;
+#pragma unroll
+  for (int i = 0; i <= N; i++) {
+    r.v[i] = make_uint4(0, 0, 0, 0);
+    if (have > 0 && i * 16 - off < have * (int)sizeof(T) && (i < N || off)) r.v[i] = base[i];
+  }
+  return r;
+}
+// Words [off / 4, off / 4 + M) of w, off bytes in: w has at least M + 4 words (M + off / 4 + 1 are read).
+template <int M, int W>
+__device__ __forceinline__ void shift_words(const uint32_t (&w)[W], int off, uint32_t (&to)[M]) {
+  static_assert(W >= M + 4, "words past the last shifted one");
+  uint32_t a[M + 2], b[M + 1];
+#pragma unroll
+  for (int i = 0; i < M + 2; i++) a[i] = off & 8 ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < M + 1; i++) b[i] = off & 4 ? a[i + 1] : a[i];
+#pragma unroll
+  for (int i = 0; i < M; i++) to[i] = __funnelshift_r(b[i], b[i + 1], (off & 3) * 8);
+}
+template <class T, int V>
+__device__ __forceinline__ Raw<T, V> shifted(const RawOdd<T, V>& r, int off, int have) {
+  constexpr int M = V * sizeof(T) / 4;
+  uint32_t w[M + 4], to[M];
+#pragma unroll
+  for (int i = 0; i < M / 4 + 1; i++) {
+    w[4 * i] = r.v[i].x;
+    w[4 * i + 1] = r.v[i].y;
+    w[4 * i + 2] = r.v[i].z;
+    w[4 * i + 3] = r.v[i].w;
+  }
+  shift_words(w, off, to);
+  if (have < V) {  // what follows the row
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      if constexpr (sizeof(T) == 4) {
+        if (j >= have) to[j] = 0;
+      } else {
+        if (j >= have) to[j / 2] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
+      }
+    }
+  }
+  Raw<T, V> out;
+#pragma unroll
+  for (int i = 0; i < M / 4; i++) out.v[i] = make_uint4(to[4 * i], to[4 * i + 1], to[4 * i + 2], to[4 * i + 3]);
+  return out;
+}
+// The counterpart for stores, by a whole warp whose lanes hold consecutive values: a lane stores the
+// aligned pieces that start in its values, the last of them ending with the next lane's first
+// values; what belongs to no whole piece of the warp's is stored value by value.
+template <class T, int V>
+__device__ __forceinline__ void store_odd(T* p, const Raw<T, V>& r, int have) {
+  constexpr int N = V * sizeof(T) / 16, M = 4 * N, es = sizeof(T);
+  const int lane = threadIdx.x & 31;
+  const int head = (int)(-reinterpret_cast<uintptr_t>(p) & 15);  // bytes before the first aligned piece
+  uint32_t w[M + 4], to[M];
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    w[4 * i] = r.v[i].x;
+    w[4 * i + 1] = r.v[i].y;
+    w[4 * i + 2] = r.v[i].z;
+    w[4 * i + 3] = r.v[i].w;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) w[M + i] = __shfl_down_sync(0xffffffffu, w[i], 1);
+  shift_words(w, head, to);
+  const T* e = reinterpret_cast<const T*>(r.v);
+  int from = 0, rest = V;  // the values that are stored one by one: [0, from) and [rest, V)
+  if (lane == 0 || head > have * es) from = head / es;
+#pragma unroll
+  for (int g = 0; g < N; g++) {
+    if (head + 16 * g + 16 <= have * es && (g < N - 1 || lane < 31 || head == 0))
+      reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p) + head)[g] = make_uint4(to[4 * g], to[4 * g + 1], to[4 * g + 2], to[4 * g + 3]);
+    else
+      rest = min(rest, (head + 16 * g) / es);
+  }
+#pragma unroll
+  for (int j = 0; j < V; j++)
+    if (j < have && (j < from || j >= rest)) p[j] = e[j];
+}
+
 // The sum of v over a row's threads (a multiple of 32, threadIdx.x of them): warp sums, then the
 // warps' sums in order. `red` belongs to the row; its barrier is 1 + threadIdx.y.
 __device__ __forceinline__ float row_sum(float v, float* red) {
@@ -85,7 +180,13 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
 // threads hold a block of 128 columns. Short rows share a CTA (threadIdx.y). With many rows
 // a CTA goes through several of them and has the next one's x and residual on their way while it
 // works on one, since sums, scales and stores leave the memory idle otherwise.
-template <class T, int V, int I>
+//
+// Measured: 16,384 x 2,560 with a residual bf16 59 us (4.9 TB/s), f32 85 us (6.4 TB/s); 512 x 1,024
+// layer norm f32 4.0 us; 1 x 2,048 2.1 us. bf16 is further from the memory's rate since its 5 warps
+// per row have as many sums, scales and conversions for half the bytes.
+//
+// Odd: x, the residual or the sum has rows that start off 16 bytes.
+template <class T, int V, int I, bool Odd>
 __global__ void __launch_bounds__(I == 4 ? 1024 : 512) norm_f8_kernel(const __grid_constant__ NormF8Params p) {
   __shared__ float red_sm[2][2][32];
   const int64_t step = (int64_t)gridDim.x * blockDim.y;
@@ -94,18 +195,31 @@ __global__ void __launch_bounds__(I == 4 ? 1024 : 512) norm_f8_kernel(const __gr
   pdl_wait();
   if (r >= p.rows) return;
   const int width = blockDim.x;
-  const bool xw = (reinterpret_cast<uintptr_t>(p.x) | (uint64_t)p.x_stride * sizeof(T)) % 16 == 0,
-             rw = (reinterpret_cast<uintptr_t>(p.residual) | (uint64_t)p.residual_stride * sizeof(T)) % 16 == 0,
-             sw = (reinterpret_cast<uintptr_t>(p.sum) | (uint64_t)p.sum_stride * sizeof(T)) % 16 == 0;
   const bool ww = reinterpret_cast<uintptr_t>(p.weight) % 16 == 0, bw = reinterpret_cast<uintptr_t>(p.bias) % 16 == 0;
-  Raw<T, V> nx[I], nr[I];
+  constexpr bool kShift = Odd && I < 4;  // the longest rows leave no registers for it: 4,096 x 10,241 f32 56 us, 70 with
+  using Piece = typename std::conditional<kShift, RawOdd<T, V>, Raw<T, V>>::type;
+  Piece nx[I], nr[I];
+  auto load = [&](const void* base, int64_t at, int have) {
+    const T* from = static_cast<const T*>(base) + at;
+    if constexpr (kShift)
+      return load_odd<T, V>(from, have);
+    else
+      return load_raw<T, V>(from, have, !Odd);
+  };
   auto fetch = [&](int64_t row) {
 #pragma unroll
     for (int i = 0; i < I; i++) {
       const int c = (threadIdx.x + i * width) * V;
-      nx[i] = load_raw<T, V>(static_cast<const T*>(p.x) + row * p.x_stride + c, p.k - c, xw);
-      if (p.residual) nr[i] = load_raw<T, V>(static_cast<const T*>(p.residual) + row * p.residual_stride + c, p.k - c, rw);
+      nx[i] = load(p.x, row * p.x_stride + c, p.k - c);
+      if (p.residual) nr[i] = load(p.residual, row * p.residual_stride + c, p.k - c);
     }
+  };
+  // A loaded piece of row r as values.
+  auto values = [&](const Piece& piece, const void* base, int64_t stride, int c) {
+    if constexpr (kShift)
+      return shifted<T, V>(piece, (int)(reinterpret_cast<uintptr_t>(static_cast<const T*>(base) + r * stride) & 15), p.k - c);
+    else
+      return piece;
   };
   constexpr bool kAhead = I < 4;  // the longest rows leave no registers for a second one
   if (kAhead) fetch(r);
@@ -118,18 +232,23 @@ __global__ void __launch_bounds__(I == 4 ? 1024 : 512) norm_f8_kernel(const __gr
     if (!kAhead) fetch(r);
 #pragma unroll
     for (int i = 0; i < I; i++) {
-      unpack(nx[i], h[i]);
+      const int c = (threadIdx.x + i * width) * V;
+      Raw<T, V> x = values(nx[i], p.x, p.x_stride, c);
+      unpack(x, h[i]);
       if (p.residual) {
         float a[V];
-        unpack(nr[i], a);
+        unpack(values(nr[i], p.residual, p.residual_stride, c), a);
 #pragma unroll
         for (int j = 0; j < V; j++) h[i][j] = h[i][j] + a[j];
-        nx[i] = pack<T, V>(h[i]);
-        unpack(nx[i], h[i]);
+        x = pack<T, V>(h[i]);
+        unpack(x, h[i]);
       }
       if (p.sum) {
-        const int c = (threadIdx.x + i * width) * V;
-        store_raw(static_cast<T*>(p.sum) + r * p.sum_stride + c, nx[i], p.k - c, sw);
+        T* to = static_cast<T*>(p.sum) + r * p.sum_stride + c;
+        if constexpr (kShift)
+          store_odd<T, V>(to, x, p.k - c);
+        else
+          store_raw<T, V>(to, x, p.k - c, !Odd);
       }
     }
     if (kAhead && r + step < p.rows) fetch(r + step);
@@ -251,12 +370,12 @@ namespace {
 
 // How a kernel's rows of `warps` warps share an SM best: rows per CTA and CTAs per SM. An SM gives
 // registers to four warps at a time, so that rows of five warps alone leave a third of it idle
-// (16384 x 2560 bf16: 4 rows of 5 warps at once 64 us, 6 in CTAs of
-// three 59 us). Asked of the runtime once per kernel and width.
+// (16384 x 2560 bf16: 4 rows of 5 warps at once 64 us, 6 in CTAs of three 59 us). Asked of the
+// runtime once per kernel and width.
 struct Shape {
   int share, ctas;
 };
-template <class T, int V, int I>
+template <class T, int V, int I, bool Odd>
 Shape shape_of(int warps) {
   static std::atomic<uint32_t> known[33];
   uint32_t v = known[warps].load(std::memory_order_relaxed);
@@ -264,7 +383,7 @@ Shape shape_of(int warps) {
     int best = 0;
     for (int share = 1; share <= 8 && share * warps * 32 <= (I == 4 ? 1024 : 512); share++) {
       int ctas = 0;
-      check_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, norm_f8_kernel<T, V, I>, share * warps * 32, 0), "occupancy");
+      check_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, norm_f8_kernel<T, V, I, Odd>, share * warps * 32, 0), "occupancy");
       if (share * ctas > best) {
         best = share * ctas;
         v = (uint32_t)share << 16 | (uint32_t)ctas;
@@ -276,10 +395,10 @@ Shape shape_of(int warps) {
   return {(int)(v >> 16), (int)(v & 0xffff)};
 }
 
-template <class T, int V, int I>
-void launch_norm(const NormF8Params& p, cudaStream_t s) {
+template <class T, int V, int I, bool Odd>
+void launch_norm_variant(const NormF8Params& p, cudaStream_t s) {
   const int warps = ((p.k + V * I - 1) / (V * I) + 31) / 32;
-  Shape sh = shape_of<T, V, I>(warps);
+  Shape sh = shape_of<T, V, I, Odd>(warps);
   // Few rows go to as many SMs as there are.
   const int64_t spread = std::max<int64_t>(1, p.rows / 148);
   if (sh.share > spread) sh.share = (int)spread;
@@ -293,7 +412,18 @@ void launch_norm(const NormF8Params& p, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  check_cuda(cudaLaunchKernelEx(&cfg, norm_f8_kernel<T, V, I>, p), "norm launch");
+  check_cuda(cudaLaunchKernelEx(&cfg, norm_f8_kernel<T, V, I, Odd>, p), "norm launch");
+}
+
+template <class T, int V, int I>
+void launch_norm(const NormF8Params& p, cudaStream_t s) {
+  auto odd = [](const void* base, int64_t stride) {
+    return base && (reinterpret_cast<uintptr_t>(base) | (uint64_t)stride * sizeof(T)) % 16 != 0;
+  };
+  if (odd(p.x, p.x_stride) || odd(p.residual, p.residual_stride) || odd(p.sum, p.sum_stride))
+    launch_norm_variant<T, V, I, true>(p, s);
+  else
+    launch_norm_variant<T, V, I, false>(p, s);
 }
 
 }  // namespace

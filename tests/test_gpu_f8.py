@@ -388,3 +388,28 @@ def test_linear_closed_during_capture(svl_lib):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("k", [1, 5, 33, 511, 513, 1025, 2561, 4097, 5637, 8191, 9001, 16385])
+def test_norm_odd_rows(svl_lib, dtype, k):
+    """Rows of every alignment, x, residual and sum differently, with what lies around the sum's rows
+    left as it was; in place too."""
+    import torch
+
+    import svl
+    t = torch_dtype(dtype)
+    g = torch.Generator(device="cuda").manual_seed(k)
+    rows = 19
+    for off, (a, b, c) in enumerate([(0, 0, 0), (1, 0, 3), (0, 7, 1), (3, 3, 3), (5, 2, 8), (8, 8, 0)]):
+        wide = lambda o: torch.randn(rows, k + o + off % 3, device="cuda", generator=g).to(t)  # noqa: E731
+        x, r, big = wide(a)[:, a:a + k], wide(b)[:, b:b + k], torch.full((rows, k + c + off % 2), 9.0, device="cuda", dtype=t)
+        want_h = (x.float() + r.float()).to(t)
+        want_q, want_s, _ = svl.add_norm_f8(want_h.contiguous() if k % 8 == 0 else torch.nn.functional.pad(want_h, (0, -k % 16))[:, :k], norm=None)
+        q, s, h = svl.add_norm_f8(x, r, norm=None, out_sum=big[:, c:c + k])
+        assert torch.equal(h, want_h) and torch.equal(s, want_s) and torch.equal(q.view(torch.uint8), want_q.view(torch.uint8))
+        around = big.clone()
+        around[:, c:c + k] = 9.0
+        assert torch.all(around == 9.0)
+        q, s, h = svl.add_norm_f8(x, r, norm=None, out_sum=x)
+        assert torch.equal(h, want_h) and torch.equal(s, want_s) and torch.equal(q.view(torch.uint8), want_q.view(torch.uint8))
