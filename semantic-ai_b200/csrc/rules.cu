@@ -85,9 +85,9 @@ constexpr int kSlotBytes = 12;    // a touched token's count, first bias entry a
 // takes less than giving slots (256 rows of 4,001 f32 tokens with all rules: 10.4 us, 11.3 with
 // slots).
 //
-// Measured: 1 row of 8,000 f32 tokens with a history of 250, 16 biases and a mask 5.7 us (2.8 without
+// Measured: 1 row of 8,000 f32 tokens with a history of 250, 16 biases and a mask 5.6 us (2.8 without
 // rules); 256 rows of 4,001 f32 with all rules 8.9 us; 192 rows of 131,072 bf16 with all rules, a
-// history of 2,048 each, 50 us, of which half is the copy: 2.1 TB/s. More warps per SM would hide
+// history of 2,048 each, 49.5 us (2.1 TB/s), 21 without any rule. More warps per SM would hide
 // more of the lists' latency, but below 64 registers the spills cost more than they bring.
 //
 // Positions are counted from the 16-byte boundary at or before the row's start ("lead" elements
