@@ -328,3 +328,52 @@ def test_norm_linear_rules_together(svl_lib, rows):
     torch.cuda.synchronize()
     for a, b in zip((h, lg, out, tok), again):
         np.testing.assert_array_equal(a, b.cpu().numpy())
+
+
+@gpu
+def test_rules_in_reference_order(svl_lib):
+    """The rules read the logits that a state in reference order gives."""
+    stt = config.stt_toy()
+    cfg = stt.transformer("q8_0")
+    gm = LanguageModel(stt, cfg, synth.stt_weights(stt, cfg, std=0.05))
+    a, b = (gm.init_state(1, reference_order=True) for _ in range(2))
+    b.set_rules(allowed=[5, 6], bias={6: 100.0})
+    audio = synth.audio_tokens(stt, 1)
+    _, la = gm.step([1], audio, a, logits=True)
+    tok, lb = gm.step([1], audio, b, logits=True)
+    assert tok[0] == 6 and lb[0, 5] == la[0, 5] and lb[0, 6] == F(la[0, 6] + F(100))
+    assert np.all(np.isneginf(np.delete(lb[0], [5, 6])))
+
+
+@gpu
+def test_first_calls_captured(svl_lib):
+    """A process whose very first calls are made while a graph is captured."""
+    import subprocess
+    import sys
+    code = """
+import torch, svl
+from svl import _lib
+lib = _lib.lib()
+w = torch.eye(256, device="cuda").to(torch.float8_e4m3fn)
+lin = svl.F8Linear(w, torch.ones(2, 2, device="cuda"))
+shapes = ((1, 256), (40, 256), (200, 256), (3000, 256))
+xs = [torch.randn(s, device="cuda") for s in shapes]
+big = [torch.randn(3, 131072, device="cuda"), torch.randn(300, 40000, device="cuda").bfloat16()]
+hist = torch.zeros(3, 9000, dtype=torch.int32, device="cuda"), torch.full((3,), 9000, dtype=torch.int32, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    outs = [lin(*svl.add_norm_f8(x, x)[:2]) for x in xs]
+    rules = [svl.logits_rules(big[0], history=hist[0], lengths=hist[1]), svl.logits_rules(big[1])]
+g.replay()
+torch.cuda.synchronize()
+for x, o in zip(xs, outs):
+    assert torch.equal(o, lin(*svl.add_norm_f8(x, x)[:2]))
+assert torch.equal(rules[0][1], svl.logits_rules(big[0], history=hist[0], lengths=hist[1])[1])
+assert torch.equal(rules[1][1].long(), big[1].float().argmax(1))
+print("captured")
+"""
+    import os
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join(sys.path))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, env=env)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
