@@ -970,10 +970,11 @@ CUtensorMap plan(F8Args& a, int tn, int br) {
   return map;
 }
 
-// Up to 64 rows. Clusters of 4 (2) as long as 200 CTAs are not exceeded and each has two blocks: the
-// SMs that a few tiles leave idle then load too (1 x 2048 x 2048: 5.2 us alone, 4.0 with 2, 3.4 with
-// 4, 3.6 with 8; 1 x 11264 x 2048, 88 tiles: 5.9 alone, 6.2 with 2, 9.6 with 4). Clusters of 8 only
-// for very long axes (1 x 2560 x 10240: 8.4 us with 4, 7.2 with 8), other sizes never won.
+// Tiles of up to 32 rows. Clusters of 4 (2) as long as 200 CTAs are not exceeded and each has two
+// blocks: the SMs that a few tiles leave idle then load too (1 x 2048 x 2048: 5.2 us alone, 4.0
+// with 2, 3.4 with 4, 3.6 with 8; 1 x 11264 x 2048, 88 tiles: 5.9 alone, 6.2 with 2, 9.6 with 4).
+// Clusters of 8 only for very long axes (1 x 2560 x 10240: 8.4 us with 4, 7.2 with 8), other sizes
+// never won.
 template <int BN>
 void launch_thin(F8Args a, cudaStream_t s) {
   const CUtensorMap map = plan(a, kF8Block, BN);
@@ -1005,20 +1006,22 @@ void launch_big(F8Args a, cudaStream_t s) {
 
 }  // namespace
 
-// Which kernel. Up to 16 rows, 32, and 64 as long as two tiles of 32 rows per matrix tile fit the
-// SMs: the matrix rows as M (64 x 2048 x 2048: 5.1 us against 7.6 as a 128 x 128 tile; 64 x 11264 x
-// 2048, 176 tiles: 9.9 against 8.9). Above, 128 x 128 tiles or 128 x 256: a wave of the larger ones
-// takes 1.55 times as long (1024 x 11264 x 2048: 35 us in 5 waves, 33 in 3; 512 x 11264 x 2048: 22 us
-// in 3, 23 in 2; 256 x 11264 x 2048: 15.5 us in 2, 13.3 in 1).
+// Which kernel. Up to 32 rows the matrix rows as M; above too, in tiles of 32 rows, as long as all of
+// them run at once and have no more than 2,112 blocks in all, two of which an SM loads about as
+// fast as one of a 128 x 128 tile, but whose tiles start, end and share a long axis faster: 147 x
+// 225 x 2048 4.3 us against 6.9, 128 x 1024 x 5632 (1,408 blocks) 6.7 against 8.7, 256 x 2048 x 2048
+// (2,048 blocks) 8.0 both, 128 x 2048 x 5632 (2,816 blocks) 9.4 against 9.0. Else 128 x 128 tiles or
+// 128 x 256: a wave of the larger ones takes 1.55 times as long (1024 x 11264 x 2048: 35 us in 5
+// waves, 33 in 3; 512 x 11264 x 2048: 22 us in 3, 23 in 2; 256 x 11264 x 2048: 15.5 us in 2, 13.3 in 1).
 void launch_f8_gemm(const F8GemmParams& p, cudaStream_t s) {
   F8Args a{};
   a.p = p;
   a.kblocks = p.m.kblocks();
-  const int64_t rt = (p.rows + kF8Block - 1) / kF8Block;
+  const int64_t rt = (p.rows + kF8Block - 1) / kF8Block, thin_tiles = (p.rows + 31) / 32 * p.m.tiles();
   const int64_t wide_waves = (rt * p.m.tiles() + kSms - 1) / kSms, big_waves = (rt * ((p.m.tiles() + 1) / 2) + kSms - 1) / kSms;
   if (p.rows <= 16)
     launch_thin<16>(a, s);
-  else if (p.rows <= 32 || (p.rows <= 64 && 2 * p.m.tiles() <= kSms))
+  else if (p.rows <= 32 || (thin_tiles <= 2 * kSms && thin_tiles * a.kblocks <= 2112))
     launch_thin<32>(a, s);
   else if (big_waves * 31 < wide_waves * 20)
     launch_big(a, s);
