@@ -89,8 +89,8 @@ __device__ __forceinline__ RawOdd<T, V> load_odd(const T* p, int have) {
   }
   return r;
 }
-// Words [off / 4, off / 4 + M) of w, off bytes in: w has at least M + 4 words (M + off / 4 + 1 are read).
-template <int M, int W>
+// Words [off / 4, off / 4 + M) of w, off bytes in (a multiple of 4 without Halves).
+template <bool Halves, int M, int W>
 __device__ __forceinline__ void shift_words(const uint32_t (&w)[W], int off, uint32_t (&to)[M]) {
   static_assert(W >= M + 4, "words past the last shifted one");
   uint32_t a[M + 2], b[M + 1];
@@ -99,7 +99,7 @@ __device__ __forceinline__ void shift_words(const uint32_t (&w)[W], int off, uin
 #pragma unroll
   for (int i = 0; i < M + 1; i++) b[i] = off & 4 ? a[i + 1] : a[i];
 #pragma unroll
-  for (int i = 0; i < M; i++) to[i] = __funnelshift_r(b[i], b[i + 1], (off & 3) * 8);
+  for (int i = 0; i < M; i++) to[i] = Halves ? __funnelshift_r(b[i], b[i + 1], (off & 3) * 8) : b[i];
 }
 template <class T, int V>
 __device__ __forceinline__ Raw<T, V> shifted(const RawOdd<T, V>& r, int off, int have) {
@@ -112,7 +112,7 @@ __device__ __forceinline__ Raw<T, V> shifted(const RawOdd<T, V>& r, int off, int
     w[4 * i + 2] = r.v[i].z;
     w[4 * i + 3] = r.v[i].w;
   }
-  shift_words(w, off, to);
+  shift_words<sizeof(T) == 2>(w, off, to);
   if (have < V) {  // what follows the row
 #pragma unroll
     for (int j = 0; j < V; j++) {
@@ -146,7 +146,7 @@ __device__ __forceinline__ void store_odd(T* p, const Raw<T, V>& r, int have) {
   }
 #pragma unroll
   for (int i = 0; i < 4; i++) w[M + i] = __shfl_down_sync(0xffffffffu, w[i], 1);
-  shift_words(w, head, to);
+  shift_words<sizeof(T) == 2>(w, head, to);
   const T* e = reinterpret_cast<const T*>(r.v);
   int from = 0, rest = V;  // the values that are stored one by one: [0, from) and [rest, V)
   if (lane == 0 || head > have * es) from = head / es;
@@ -185,9 +185,14 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
 // layer norm f32 4.0 us; 1 x 2,048 2.1 us. bf16 is further from the memory's rate since its 5 warps
 // per row have as many sums, scales and conversions for half the bytes.
 //
+// The compiler's choice of registers is left to it but for odd bf16 rows of one piece, for which it
+// would take too few (16,384 x 727: 47 us, 38.5 with all that one CTA may have; aligned rows: 28).
+template <class T, int I, bool Odd>
+constexpr int kOneCta = Odd && sizeof(T) == 2 && I == 1 ? 1 : 0;
+
 // Odd: x, the residual or the sum has rows that start off 16 bytes.
 template <class T, int V, int I, bool Odd>
-__global__ void __launch_bounds__(I == 4 ? 1024 : 512) norm_f8_kernel(const __grid_constant__ NormF8Params p) {
+__global__ void __launch_bounds__(I == 4 ? 1024 : 512, kOneCta<T, I, Odd>) norm_f8_kernel(const __grid_constant__ NormF8Params p) {
   __shared__ float red_sm[2][2][32];
   const int64_t step = (int64_t)gridDim.x * blockDim.y;
   int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
@@ -221,7 +226,9 @@ __global__ void __launch_bounds__(I == 4 ? 1024 : 512) norm_f8_kernel(const __gr
     else
       return piece;
   };
-  constexpr bool kAhead = I < 4;  // the longest rows leave no registers for a second one
+  // Two pieces of f32 leave no registers for a second row and a second CTA, which is worth more
+  // (3,276 x 5,120: 53 us with the next row ahead, 40 without); four leave none at all.
+  constexpr bool kAhead = I == 1 || (I == 2 && (Odd || sizeof(T) == 2));
   if (kAhead) fetch(r);
   for (int turn = 0; r < p.rows; r += step, turn ^= 1) {
     // A CTA's rows use disjoint parts of red (blockDim.x / 32 * blockDim.y <= 32 warps), and a row
@@ -428,12 +435,12 @@ void launch_norm(const NormF8Params& p, cudaStream_t s) {
 
 }  // namespace
 
-// 32 bytes of the stream per thread and piece, 16 of short bf16 rows (16384 x 256: 8 us against
-// 14) and of rows too long for 1,024 threads and two pieces.
+// 32 bytes of the stream per thread and piece, 16 of bf16 rows that half a warp would hold (16384 x
+// 256: 8 us against 14) and of rows too long for 1,024 threads and two pieces.
 void launch_norm_f8(const NormF8Params& p, cudaStream_t s) {
   using B = __nv_bfloat16;
   if (p.bf16) {
-    if (p.k <= 512)
+    if (p.k <= 256)
       launch_norm<B, 8, 1>(p, s);
     else if (p.k <= 8192)
       launch_norm<B, 16, 1>(p, s);
