@@ -198,6 +198,20 @@ def test_linear(svl_lib, rows, n, k, out):
     lin.check()
 
 
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,n,k", [(256, 1024, 6400), (300, 1000, 5000), (140, 1200, 2900), (147, 225, 2048), (290, 130, 700), (1000, 300, 300)])
+def test_linear_few_tiles(svl_lib, rows, n, k, out):
+    """More than 64 rows with few tiles, small ones and those that CTAs share; two runs give the same bits."""
+    import torch
+
+    import svl
+    d = quantised(rows, k, n, rows + k, bias=True)
+    lin = svl.F8Linear(d["w"], d["ws"], d["b"])
+    got = lin(d["q"], d["s"], out_dtype=torch_dtype(out))
+    check_linear(got, d, out)
+    assert torch.equal(got, lin(d["q"], d["s"], out_dtype=torch_dtype(out)))
+
+
 @pytest.mark.parametrize("rows", [1, 20, 200])
 def test_linear_padded(svl_lib, rows):
     """Rows with NaN codes between them, scales in a wider table, outputs in a wider table whose
@@ -219,7 +233,7 @@ def test_linear_padded(svl_lib, rows):
 
 
 @pytest.mark.parametrize("out", ["f32", "bf16"])
-@pytest.mark.parametrize("rows,n,k", [(100, 131, 8200), (128, 4001, 2500), (129, 257, 2600), (65, 135, 6000), (130, 8, 5000)])
+@pytest.mark.parametrize("rows,n,k", [(100, 131, 8200), (128, 4001, 2500), (129, 257, 2600), (65, 135, 6000), (130, 8, 5000), (300, 1031, 6000)])
 def test_linear_odd_outputs(svl_lib, rows, n, k, out):
     """Outputs of an odd width at an odd offset, also where CTAs share a tile; nothing outside is written."""
     import torch
