@@ -425,16 +425,18 @@ int64_t clusters_at_once(int n) {
 // CTAs per row. One where it has at most 16,384 tokens to go through: a cluster costs more than its
 // share of the work saves. Up to 148 rows: the most that still run at once with an SM each (16
 // rows of 131,072 bf16 tokens without rules: 6 CTAs 4.3 us, 8 in two waves 7.4; 64 rows: 2 CTAs
-// 7.2, 8 CTAs 8.3). More rows: the number whose waves take the shortest, the lists and the
+// 7.2, 8 CTAs 8.3). Where that is one CTA, two of a half each per SM for rows with lists, if they run
+// at once (120 rows of 50,257 f32 tokens, a history of 500: 25 us with one, 20 with two). More rows: the number whose waves take the shortest, the lists and the
 // joining of a CTA's results counted like 12,000 tokens (192 rows of 131,072 bf16 tokens with all
 // rules: 5 CTAs 52 us, 2 CTAs 54, 8 CTAs 59, 1 CTA 85; 512 rows of 32,000: 1 CTA 11.3, 2 CTAs 14.3).
 template <class T>
-int rules_split(int64_t rows, int64_t span) {
+int rules_split(int64_t rows, int64_t span, bool lists) {
   if (span <= 16384) return 1;
   int split = 1;
   if (rows <= 148) {
     for (int n = 2; n <= 8; n++)
       if (rows <= clusters_at_once<rules_kernel<T, 512, 1>, 512, 1>(n)) split = n;
+    if (split == 1 && lists && rows <= clusters_at_once<rules_kernel<T, 512, 2>, 512, 2>(2)) split = 2;
     return split;
   }
   int64_t least = INT64_MAX;
@@ -454,7 +456,7 @@ void launch_rules(const RulesParams& p, cudaStream_t s) {
   const int ve = p.bf16 ? 8 : 4;
   const int64_t span = (int64_t)p.vocab + ve - 1;  // with the lead of the worst row
   const int entries = (p.rules.d_history ? p.rules.history_cap : 0) + (p.rules.d_bias_ids ? p.rules.bias_cap : 0);
-  const int split = p.bf16 ? rules_split<__nv_bfloat16>(p.rows, span) : rules_split<float>(p.rows, span);
+  const int split = p.bf16 ? rules_split<__nv_bfloat16>(p.rows, span, entries) : rules_split<float>(p.rows, span, entries);
   const int range = (int)((span + split - 1) / split + 31) / 32 * 32;
   const int chunk = std::min(range, entries > kLongLists ? kMaxChunkLong : kMaxChunk);
   // Two pieces per thread; 512 threads where two CTAs per SM take all rows (256 rows of 4,001 f32

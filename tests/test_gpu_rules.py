@@ -231,7 +231,8 @@ def test_only_tokens_or_only_logits(svl_lib):
     (1, 1100001, 700, 5, "bf16"),      # chunks without room for a whole eighth
     (150, 20001, 60, 9, "bf16"),       # more rows than SMs
     (300, 16390, 2100, 0, "f32"),      # history entries past the first in flight
-    (33, 131072, 40, 8, "bf16")])
+    (33, 131072, 40, 8, "bf16"),
+    (120, 17001, 50, 9, "f32")])       # two CTAs per SM
 @pytest.mark.parametrize("in_place", [False, True])
 def test_splits_and_chunks(svl_lib, rows, vocab, history, biased, dtype, in_place):
     g, r = make(rows, vocab, rows + vocab, history=history, biased=biased, dense=True, masks=2)
