@@ -13,16 +13,32 @@
 namespace svl {
 namespace {
 
-// V consecutive values of a row as they lie in memory; `have` of them exist. `wide`: the row starts
-// on 16 bytes.
+// V consecutive values of a row as they lie in memory; `have` of them exist. `wide`: they start on 16
+// bytes, `wider`: on 32.
 template <class T, int V>
 struct Raw {
   uint4 v[V * sizeof(T) / 16];
 };
+// 32 bytes per lane, 32-byte aligned. Two loads of 16 with 16 between the lanes' would each touch
+// twice the lines.
+__device__ __forceinline__ void load32(const void* p, uint4& a, uint4& b) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+               : "l"(p));
+}
+__device__ __forceinline__ void store32(void* p, const uint4& a, const uint4& b) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w),
+               "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
+}
 template <class T, int V>
-__device__ __forceinline__ Raw<T, V> load_raw(const T* p, int have, bool wide) {
+__device__ __forceinline__ Raw<T, V> load_raw(const T* p, int have, bool wide, bool wider) {
+  constexpr int N = V * sizeof(T) / 16;
   Raw<T, V> r;
-  if (wide && have >= V) {
+  if (N % 2 == 0 && wider && have >= V) {
+#pragma unroll
+    for (int i = 0; i + 1 < N; i += 2) load32(reinterpret_cast<const uint4*>(p) + i, r.v[i], r.v[i + 1]);
+  } else if (wide && have >= V) {
 #pragma unroll
     for (int i = 0; i < (int)(V * sizeof(T) / 16); i++) r.v[i] = reinterpret_cast<const uint4*>(p)[i];
   } else {
@@ -33,8 +49,12 @@ __device__ __forceinline__ Raw<T, V> load_raw(const T* p, int have, bool wide) {
   return r;
 }
 template <class T, int V>
-__device__ __forceinline__ void store_raw(T* p, const Raw<T, V>& r, int have, bool wide) {
-  if (wide && have >= V) {
+__device__ __forceinline__ void store_raw(T* p, const Raw<T, V>& r, int have, bool wide, bool wider) {
+  constexpr int N = V * sizeof(T) / 16;
+  if (N % 2 == 0 && wider && have >= V) {
+#pragma unroll
+    for (int i = 0; i + 1 < N; i += 2) store32(reinterpret_cast<uint4*>(p) + i, r.v[i], r.v[i + 1]);
+  } else if (wide && have >= V) {
 #pragma unroll
     for (int i = 0; i < (int)(V * sizeof(T) / 16); i++) reinterpret_cast<uint4*>(p)[i] = r.v[i];
   } else {
@@ -181,18 +201,18 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
 // a CTA goes through several of them and has the next one's x and residual on their way while it
 // works on one, since sums, scales and stores leave the memory idle otherwise.
 //
-// Measured: 16,384 x 2,560 with a residual bf16 59 us (4.9 TB/s), f32 85 us (6.4 TB/s); 512 x 1,024
-// layer norm f32 4.0 us; 1 x 2,048 2.1 us. bf16 is further from the memory's rate since its 5 warps
-// per row have as many sums, scales and conversions for half the bytes.
+// Measured with a residual: 16,384 x 2,560 bf16 48 us (6.2 TB/s; 59 with loads of 16 bytes, which made
+// L1 the bound), 8,192 x 2,048 f32 35 us (6.2 TB/s); 512 x 1,024 layer norm f32 3.8 us; 1 x 2,048 2.1 us.
 //
-// The compiler's choice of registers is left to it but for odd bf16 rows of one piece, for which it
-// would take too few (16,384 x 727: 47 us, 38.5 with all that one CTA may have; aligned rows: 28).
+// The compiler's choice of registers is left to it but for bf16 rows of one piece. For odd ones it would
+// take too few (16,384 x 727: 47 us, 38.5 with all that one CTA may have; aligned rows: 28); for
+// aligned ones too many (3,276 x 5,120: 36.5 us with 103, 23.2 with 64).
 template <class T, int I, bool Odd>
-constexpr int kOneCta = Odd && sizeof(T) == 2 && I == 1 ? 1 : 0;
+constexpr int kLeastCtas = sizeof(T) == 2 && I == 1 ? (Odd ? 1 : 2) : 0;
 
 // Odd: x, the residual or the sum has rows that start off 16 bytes.
 template <class T, int V, int I, bool Odd>
-__global__ void __launch_bounds__(I == 4 ? 1024 : 512, kOneCta<T, I, Odd>) norm_f8_kernel(const __grid_constant__ NormF8Params p) {
+__global__ void __launch_bounds__(I == 4 ? 1024 : 512, kLeastCtas<T, I, Odd>) norm_f8_kernel(const __grid_constant__ NormF8Params p) {
   __shared__ float red_sm[2][2][32];
   const int64_t step = (int64_t)gridDim.x * blockDim.y;
   int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
@@ -200,23 +220,25 @@ __global__ void __launch_bounds__(I == 4 ? 1024 : 512, kOneCta<T, I, Odd>) norm_
   pdl_wait();
   if (r >= p.rows) return;
   const int width = blockDim.x;
-  const bool ww = reinterpret_cast<uintptr_t>(p.weight) % 16 == 0, bw = reinterpret_cast<uintptr_t>(p.bias) % 16 == 0;
+  const bool ww = reinterpret_cast<uintptr_t>(p.weight) % 32 == 0, bw = reinterpret_cast<uintptr_t>(p.bias) % 32 == 0;
+  auto on32 = [](const void* base, int64_t stride) { return (reinterpret_cast<uintptr_t>(base) | (uint64_t)stride * sizeof(T)) % 32 == 0; };
+  const bool x32 = on32(p.x, p.x_stride), r32 = on32(p.residual, p.residual_stride), s32 = on32(p.sum, p.sum_stride);
   constexpr bool kShift = Odd && I < 4;  // the longest rows leave no registers for it: 4,096 x 10,241 f32 56 us, 70 with
   using Piece = typename std::conditional<kShift, RawOdd<T, V>, Raw<T, V>>::type;
   Piece nx[I], nr[I];
-  auto load = [&](const void* base, int64_t at, int have) {
+  auto load = [&](const void* base, int64_t at, int have, bool wider) {
     const T* from = static_cast<const T*>(base) + at;
     if constexpr (kShift)
       return load_odd<T, V>(from, have);
     else
-      return load_raw<T, V>(from, have, !Odd);
+      return load_raw<T, V>(from, have, !Odd, !Odd && I < 4 && wider);
   };
   auto fetch = [&](int64_t row) {
 #pragma unroll
     for (int i = 0; i < I; i++) {
       const int c = (threadIdx.x + i * width) * V;
-      nx[i] = load(p.x, row * p.x_stride + c, p.k - c);
-      if (p.residual) nr[i] = load(p.residual, row * p.residual_stride + c, p.k - c);
+      nx[i] = load(p.x, row * p.x_stride + c, p.k - c, x32);
+      if (p.residual) nr[i] = load(p.residual, row * p.residual_stride + c, p.k - c, r32);
     }
   };
   // A loaded piece of row r as values.
@@ -255,7 +277,7 @@ __global__ void __launch_bounds__(I == 4 ? 1024 : 512, kOneCta<T, I, Odd>) norm_
         if constexpr (kShift)
           store_odd<T, V>(to, x, p.k - c);
         else
-          store_raw<T, V>(to, x, p.k - c, !Odd);
+          store_raw<T, V>(to, x, p.k - c, !Odd, !Odd && I < 4 && s32);
       }
     }
     if (kAhead && r + step < p.rows) fetch(r + step);
@@ -287,12 +309,12 @@ __global__ void __launch_bounds__(I == 4 ? 1024 : 512, kOneCta<T, I, Odd>) norm_
         for (int j = 0; j < V; j++) h[i][j] = h[i][j] * rstd;
         float a8[V];
         if (p.weight) {
-          unpack(load_raw<float, V>(p.weight + c, have, ww), a8);
+          unpack(load_raw<float, V>(p.weight + c, have, false, ww), a8);
 #pragma unroll
           for (int j = 0; j < V; j++) h[i][j] = h[i][j] * a8[j];
         }
         if (p.bias && p.norm == NORM_LAYER) {
-          unpack(load_raw<float, V>(p.bias + c, have, bw), a8);
+          unpack(load_raw<float, V>(p.bias + c, have, false, bw), a8);
 #pragma unroll
           for (int j = 0; j < V; j++) h[i][j] = h[i][j] + a8[j];
         }
@@ -377,7 +399,7 @@ namespace {
 
 // How a kernel's rows of `warps` warps share an SM best: rows per CTA and CTAs per SM. An SM gives
 // registers to four warps at a time, so that rows of five warps alone leave a third of it idle
-// (16384 x 2560 bf16: 4 rows of 5 warps at once 64 us, 6 in CTAs of three 59 us). Asked of the
+// (16384 x 2560 bf16: 4 rows of 5 warps at once 8 % slower than 6 in CTAs of three). Asked of the
 // runtime once per kernel and width.
 struct Shape {
   int share, ctas;
