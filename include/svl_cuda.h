@@ -405,7 +405,9 @@ SVL_API svl_status svl_rvq_encode_device(svl_rvq* rvq, int32_t batch, int32_t fr
  * `device` is the GPU that holds the tensors (it need not be the current one, which a call leaves
  * as it was), `cuda_stream` a stream of it (NULL = its default stream). Calls only enqueue work,
  * allocate nothing and may be captured into graphs; zero rows are no work. Strides count
- * elements. Outputs must not overlap inputs except where a call says so. */
+ * elements. Outputs must not overlap inputs except where a call says so. Pointers start on a
+ * multiple of their elements' size (SVL_ERR_INVALID_INPUT otherwise). A matrix has to outlive the
+ * graphs that captured its products. */
 
 /* h = x + residual; y = norm(h); y as e4m3 rows.
  *   d_x, d_residual (NULL = none), d_sum (h; NULL = not kept): [rows][k] of `dtype`

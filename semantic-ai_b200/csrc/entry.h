@@ -34,6 +34,12 @@ inline void require(bool ok, const char* msg, svl_status code = SVL_ERR_INVALID_
   if (!ok) throw Error(code, msg);
 }
 
+// Every pointer that is given starts on a multiple of its elements' size.
+template <class... P>
+void require_aligned(size_t size, P... pointers) {
+  require(((reinterpret_cast<uintptr_t>(pointers) % size == 0) && ...), "a pointer is not aligned to its elements");
+}
+
 // `device` current for the life of the guard, the caller's device again afterwards: the
 // operators work on tensors of any device, whichever is current.
 class OnDevice {

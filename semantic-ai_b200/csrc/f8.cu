@@ -555,6 +555,8 @@ SVL_API svl_status svl_add_norm_f8_device(int32_t device, int64_t rows, int32_t 
     require(reinterpret_cast<uintptr_t>(d_q) % 16 == 0, "d_q must be 16-byte aligned");
     require(scale_stride >= rows, "scale_stride is below the row count");
     require(eps >= 0.f, "eps must not be negative");
+    svl::require_aligned(dtype == SVL_DT_F32 ? 4 : 2, d_x, d_residual, d_sum);
+    svl::require_aligned(4, d_weight, d_bias, d_scales);
     OnDevice on(device);
     svl::NormF8Params p{};
     p.x = d_x;
@@ -617,6 +619,7 @@ SVL_API svl_status svl_f8_linear_create_device(int32_t n, int32_t k, const uint8
     *out = nullptr;
     check_sizes(n, k);
     require(weight_stride >= k, "weight_stride is below k");
+    svl::require_aligned(4, d_scales, d_bias);
     check_device(device);
     OnDevice on(device);
     auto L = std::make_unique<svl_f8_linear>();
@@ -658,6 +661,8 @@ SVL_API svl_status svl_f8_linear_device(svl_f8_linear* linear, int64_t rows, con
     require(reinterpret_cast<uintptr_t>(d_q) % 16 == 0, "d_q must be 16-byte aligned");
     require(scale_stride >= rows, "scale_stride is below the row count");
     require(out_stride >= linear->m.n, "out_stride is below n");
+    svl::require_aligned(4, d_scales);
+    svl::require_aligned(out_dtype == SVL_DT_F32 ? 4 : 2, d_out);
     OnDevice on(linear->device);
     svl::F8GemmParams p{};
     p.m = linear->m;

@@ -525,6 +525,9 @@ extern "C" SVL_API svl_status svl_logits_rules_device(int32_t device, int64_t ro
     if (rows == 0) return;
     require(d_logits && (d_out || d_tokens || R.append), "null argument");
     require(logits_stride >= vocab && (!d_out || out_stride >= vocab), "a row stride is below vocab");
+    svl::require_aligned(dtype == SVL_DT_F32 ? 4 : 2, d_logits, d_out);
+    svl::require_aligned(4, d_tokens, R.d_history, R.d_lengths, R.d_repetition, R.d_frequency, R.d_presence,
+                         R.d_dense_bias, R.d_bias_ids, R.d_bias_values, R.d_masks, R.d_mask_rows);
     svl::OnDevice on(device);
     p.rows = rows;
     p.vocab = vocab;

@@ -103,3 +103,27 @@ def test_state_rules_refuse_without_a_state(svl_lib):
     from svl import _lib
     with pytest.raises(_lib.SvlError, match="null state"):
         _lib.check(svl_lib.svl_state_set_rules(None, -1, None))
+
+
+@pytest.mark.parametrize("change", [dict(x=PTR + 2), dict(dtype=1, x=PTR + 1), dict(res=PTR + 2, rs=256), dict(sum=PTR + 1, ss=256),
+                                    dict(w=PTR + 2), dict(b=PTR + 1), dict(scales=PTR + 2)])
+def test_norm_refuses_misaligned(svl_lib, change):
+    assert norm(svl_lib, **change) == INVALID
+    assert b"aligned" in svl_lib.svl_last_error()
+
+
+@pytest.mark.parametrize("change", [
+    dict(logits=PTR + 2), dict(dtype=1, logits=PTR + 1), dict(out=PTR + 2), dict(tokens=PTR + 2), dict(d_dense_bias=PTR + 1),
+    dict(d_history=PTR + 2, d_lengths=PTR, history_cap=8, history_stride=8), dict(d_history=PTR, d_lengths=PTR + 2, history_cap=8, history_stride=8),
+    dict(d_bias_ids=PTR + 1, d_bias_values=PTR, bias_cap=4, bias_stride=4), dict(d_bias_ids=PTR, d_bias_values=PTR + 2, bias_cap=4, bias_stride=4),
+    dict(d_masks=PTR + 2, n_masks=4, mask_stride=4), dict(d_mask_rows=PTR + 1), dict(d_repetition=PTR + 2)])
+def test_rules_refuse_misaligned(svl_lib, change):
+    assert rules(svl_lib, **change) == INVALID
+    assert b"aligned" in svl_lib.svl_last_error()
+
+
+def test_linear_create_refuses_misaligned(svl_lib):
+    h = ctypes.c_void_p()
+    for s, b in ((PTR + 2, None), (PTR, PTR + 1)):
+        assert svl_lib.svl_f8_linear_create_device(128, 128, PTR, 128, s, b, 0, None, ctypes.byref(h)) == INVALID
+        assert b"aligned" in svl_lib.svl_last_error()
