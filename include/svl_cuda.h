@@ -416,8 +416,10 @@ SVL_API svl_status svl_rvq_encode_device(svl_rvq* rvq, int32_t batch, int32_t fr
  *   norm_kind: SVL_NORM_RMS (h / sqrt(mean(h^2) + eps) * weight), SVL_NORM_LAYER
  *   ((h - mean) / sqrt(var + eps) * weight + bias) or -1 (y = h); d_weight and d_bias are f32
  *   [k], NULL = ones and zeros.
- *   Per block: a = max(max |y|, 2^-100), scale = a / 448, q = e4m3(y * (448 / a)), rounded to
- *   nearest even. A block that holds a NaN or an infinity stands for NaN.
+ *   Per block: a = max(max |y|, 2^-100), scale = a / 448, q = e4m3(y * 448 / a), to nearest even.
+ *   Without a norm the quotient is rounded once before (to f32), so that a y of few bits, as in bf16
+ *   rows, gets the nearest e4m3 value; with one, 448 / a and the product are rounded. A block that
+ *   holds a NaN or an infinity stands for NaN.
  * q_stride is a multiple of 16 bytes (svl_f8_linear_device reads the rows with TMA), k at most
  * 32,768 (SVL_ERR_UNSUPPORTED above). Columns [k, q_stride) are left as they were. */
 SVL_API svl_status svl_add_norm_f8_device(int32_t device, int64_t rows, int32_t k, int32_t dtype,
@@ -433,7 +435,7 @@ SVL_API svl_status svl_add_norm_f8_device(int32_t device, int64_t rows, int32_t 
  * out for svl_f8_linear_device. Immutable; may be shared by threads and streams. */
 typedef struct svl_f8_linear svl_f8_linear;
 /* From host f32 tensors "weight" [n][k] and (optional) "bias" [n]: scale = max(max |w|, 2^-100)
- * / 448 of the block, q = e4m3(w * (448 / max)), rounded to nearest even. */
+ * / 448 of the block, q = e4m3(w * 448 / max), the quotient rounded once before. */
 SVL_API svl_status svl_f8_linear_create(int32_t n, int32_t k, const svl_tensor_view* tensors,
                                         int32_t n_tensors, int32_t device, svl_f8_linear** out);
 /* From e4m3 weights on the device: d_weight [n] rows, weight_stride bytes apart, d_scales

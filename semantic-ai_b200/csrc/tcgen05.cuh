@@ -122,6 +122,11 @@ __device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
 __device__ __forceinline__ void fma_pair(uint64_t& acc, uint64_t a, uint64_t b) {
   asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
 }
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ float pair_lo(uint64_t v) { return __uint_as_float((uint32_t)v); }
 __device__ __forceinline__ float pair_hi(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t columns) {
