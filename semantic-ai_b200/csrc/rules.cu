@@ -70,6 +70,47 @@ constexpr int kDirect = 8192;          // tokens of a chunk that has counts for 
 constexpr int kAhead = 4;         // 16-byte loads of logits a thread has in flight
 constexpr int kSettle = 2;        // touched tokens whose logits a thread has in flight over the stream
 constexpr int kSlotBytes = 12;    // a touched token's count, first bias entry and position
+constexpr uint32_t kRepeated = 1u << 31;  // in the place of a first entry: the token has several
+
+// Adds the sparse biases of tokens with several entries to their values, in the entries' order, by one warp: 32
+// entries at a time, of which those of one token are added lane by lane. Linear in the list, whatever repeats
+// (every such token walking the list for itself: one row of 131,072 tokens, 8,192 entries of which one id is there
+// twice, 764 us).
+__device__ __forceinline__ void add_repeated(const int32_t* ids, const float* vals, int listed, int from, int to, int v0, bool direct,
+                                          const uint32_t* first, const uint32_t* touched, const uint32_t* word_slot, uint32_t* value) {
+  constexpr uint32_t kAll = 0xffffffffu;
+  constexpr int kBatches = 8;  // ids of 256 entries in flight
+  const int lane = threadIdx.x;
+  for (int k0 = 0; k0 < listed; k0 += kBatches * 32) {
+    int id[kBatches];
+#pragma unroll
+    for (int j = 0; j < kBatches; j++) id[j] = k0 + j * 32 + lane < listed ? ids[k0 + j * 32 + lane] : -1;
+#pragma unroll 1
+    for (int j = 0; j < kBatches; j++) {
+      int at = -1;
+      if (id[0] >= from && id[0] < to) {
+        const int u = id[0] - v0;
+        at = direct ? u : (int)word_slot[u >> 5] + __popc(touched[u >> 5] & ((1u << (u & 31)) - 1));
+        if (first[at] != kRepeated) at = -1;
+      }
+      if (__any_sync(kAll, at >= 0)) {
+        const float v = at >= 0 ? vals[k0 + j * 32 + lane] : 0.f;
+        const uint32_t same = __match_any_sync(kAll, at);
+        float sum = at >= 0 ? __uint_as_float(value[at]) : 0.f;
+        uint32_t rest = at >= 0 ? same : 0;
+        while (__any_sync(kAll, rest != 0)) {
+          const float x = __shfl_sync(kAll, v, rest ? __ffs((int)rest) - 1 : lane);
+          if (rest) sum = sum + x;
+          rest &= rest - 1;
+        }
+        if (at >= 0 && __ffs((int)same) - 1 == lane) value[at] = __float_as_uint(sum);
+        __syncwarp();
+      }
+#pragma unroll
+      for (int i = 0; i + 1 < kBatches; i++) id[i] = id[i + 1];
+    }
+  }
+}
 
 // Bound by HBM for many tokens, by a chain of a few dependent loads for few. A row is shared by the
 // CTAs of a cluster, each with a contiguous range of the vocabulary, taken in chunks (one, up to
@@ -111,7 +152,7 @@ __global__ void __launch_bounds__(Threads, PerSm) rules_kernel(const __grid_cons
   if (split > 1) cluster_arrive();  // waited for before the ranks' shared memory is written
   pdl_launch();
   pdl_wait();
-  uint32_t* first = count + slots;  // 65,536 minus the first entry's index, 0: none
+  uint32_t* first = count + slots;  // 65,536 minus the first entry's index, 0: none, or kRepeated
   int* list = reinterpret_cast<int*>(first + slots);
   uint32_t* touched = first + 2 * slots;       // [chunk / 32]
   uint32_t* word_slot = touched + chunk / 32;  // [chunk / 32]
@@ -171,7 +212,8 @@ __global__ void __launch_bounds__(Threads, PerSm) rules_kernel(const __grid_cons
     const bool table = said || listed;
     int n = 0;  // touched tokens
     float mine[kSettle], mine_dense[kSettle];
-    // A touched token's value up to the grammar, of its logit and dense bias.
+    // A touched token's value up to the grammar, of its logit and dense bias; without the sparse biases
+    // where it has several.
     auto settled = [&](int i, float l, float d) {
       const int at = direct ? list[i] : i;
       const uint32_t c = count[at], f = first[at];
@@ -180,16 +222,7 @@ __global__ void __launch_bounds__(Threads, PerSm) rules_kernel(const __grid_cons
         l = l - (penalty[1] * (float)c + penalty[2]);
       }
       if (dense) l = l + d;
-      if (f) {
-        const int entry = 65536 - (int)f;
-        l = l + vals[entry];
-        if (twice) {
-          const int v = v0 + list[i];
-          for (int k = entry + 1; k < listed; k++)
-            if (ids[k] == v) l = l + vals[k];
-        }
-      }
-      return l;
+      return f && f != kRepeated ? l + vals[65536 - (int)f] : l;
     };
     if (table) {
       const int from = max(v0, 0), to = c1 - lead;      // the chunk's tokens
@@ -220,11 +253,16 @@ __global__ void __launch_bounds__(Threads, PerSm) rules_kernel(const __grid_cons
         if (*reinterpret_cast<volatile uint32_t*>(&touched[at >> 5]) & bit) return false;
         return !(atomicOr(&touched[at >> 5], bit) & bit);
       };
+      auto bias = [&](int i, int at) {
+        if (!atomicMax(&first[at], 65536u - i)) return;
+        atomicMax(&first[at], kRepeated);
+        twice = 1;
+      };
       if (direct) {
         auto add = [&](int at) {
           if (touch(at)) list[atomicAdd(&touched_n, 1)] = at;
         };
-        entries([&](int i, int at) { add(at); if (atomicMax(&first[at], 65536u - i)) twice = 1; },
+        entries([&](int i, int at) { add(at); bias(i, at); },
                 [&](int at) { add(at); atomicAdd(&count[at], 1u); });
         __syncthreads();
       } else {
@@ -242,7 +280,7 @@ __global__ void __launch_bounds__(Threads, PerSm) rules_kernel(const __grid_cons
         }
         __syncthreads();
         auto slot = [&](int at) { return word_slot[at >> 5] + __popc(touched[at >> 5] & ((1u << (at & 31)) - 1)); };
-        entries([&](int i, int at) { if (atomicMax(&first[slot(at)], 65536u - i)) twice = 1; },
+        entries([&](int i, int at) { bias(i, slot(at)); },
                 [&](int at) { atomicAdd(&count[slot(at)], 1u); });
       }
       n = touched_n;
@@ -354,9 +392,24 @@ __global__ void __launch_bounds__(Threads, PerSm) rules_kernel(const __grid_cons
         if (out) store_logit(out + v, l);
         best = max_key(best, pick_key(l, v));
       };
+      if (twice) {
+        // The values of tokens with several entries stand in the place of their counts now.
 #pragma unroll
-      for (int j = 0; j < kSettle; j++)
-        if (t + j * threads < n) put(t + j * threads, settled(t + j * threads, mine[j], mine_dense[j]));
+        for (int j = 0; j < kSettle; j++) {
+          const int i = t + j * threads, at = i < n ? direct ? list[i] : i : 0;
+          if (i < n && first[at] == kRepeated) count[at] = __float_as_uint(settled(i, mine[j], mine_dense[j]));
+        }
+        __syncthreads();
+        if (t < 32) add_repeated(ids, vals, listed, max(v0, 0), c1 - lead, v0, direct, first, touched, word_slot, count);
+        __syncthreads();
+      }
+#pragma unroll
+      for (int j = 0; j < kSettle; j++) {
+        const int i = t + j * threads;
+        if (i >= n) break;
+        const int at = direct ? list[i] : i;
+        put(i, first[at] == kRepeated ? __uint_as_float(count[at]) : settled(i, mine[j], mine_dense[j]));
+      }
       for (int i = t + kSettle * threads; i < n; i += threads) put(i, __uint_as_float(count[direct ? list[i] : i]));
     }
   }
