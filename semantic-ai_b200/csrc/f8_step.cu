@@ -283,41 +283,47 @@ void state_set_rules(State& s, int stream, const svl_stt_rules* rules) {
     check_cuda(cudaMemsetAsync(s.said_len.p, 0, s.said_len.bytes, st), "memset");
     check_cuda(cudaMemsetAsync(s.said.p, 0xff, s.said.bytes, st), "memset");
   }
-  // Without rules: no penalty, no entry, no grammar.
-  std::vector<int32_t> ids(SVL_RULES_BIASES, -1);
-  std::vector<float> vals(SVL_RULES_BIASES, 0.f);
-  const float rep = rules ? rules->repetition : 1.f, freq = rules ? rules->frequency : 0.f, pres = rules ? rules->presence : 0.f;
-  for (int i = 0; rules && i < rules->n_bias; i++) {
-    ids[i] = (int32_t)rules->bias_ids[i];
-    vals[i] = rules->bias_values[i];
+  // The rules of streams [lo, hi), all of them the first time; without rules: no penalty, no entry, no grammar.
+  const bool first_time = !s.rules;
+  const int lo = first_time || stream < 0 ? 0 : stream, hi = first_time || stream < 0 ? B : stream + 1, n = hi - lo;
+  std::vector<float> rep(n, 1.f), freq(n, 0.f), pres(n, 0.f), vals((size_t)n * SVL_RULES_BIASES, 0.f);
+  std::vector<int32_t> ids((size_t)n * SVL_RULES_BIASES, -1), rows(n, -1);
+  std::vector<uint32_t> masks(rules && rules->allowed ? (size_t)n * words : 0);
+  for (int b = lo; rules && b < hi; b++) {
+    if (stream >= 0 && b != stream) continue;
+    const int at = b - lo;
+    rep[at] = rules->repetition;
+    freq[at] = rules->frequency;
+    pres[at] = rules->presence;
+    for (int i = 0; i < rules->n_bias; i++) {
+      ids[(size_t)at * SVL_RULES_BIASES + i] = (int32_t)rules->bias_ids[i];
+      vals[(size_t)at * SVL_RULES_BIASES + i] = rules->bias_values[i];
+    }
+    if (!rules->allowed) continue;
+    rows[at] = b;
+    std::copy(rules->allowed, rules->allowed + words, masks.begin() + (size_t)at * words);
   }
-  auto put = [&](int b, bool plain) {
-    const float one = 1.f, zero = 0.f;
-    const int32_t row = !plain && rules && rules->allowed ? b : -1;
-    auto up = [&](DevBuf& to, int64_t at, const void* from, int64_t bytes) {
-      check_cuda(cudaMemcpyAsync(to.as<uint8_t>() + at, from, bytes, cudaMemcpyHostToDevice, st), "upload");
-    };
-    const std::vector<int32_t> none(plain ? SVL_RULES_BIASES : 0, -1);
-    up(s.rule_rep, b * 4ll, plain ? &one : &rep, 4);
-    up(s.rule_freq, b * 4ll, plain ? &zero : &freq, 4);
-    up(s.rule_pres, b * 4ll, plain ? &zero : &pres, 4);
-    up(s.rule_ids, (int64_t)b * SVL_RULES_BIASES * 4, plain ? none.data() : ids.data(), SVL_RULES_BIASES * 4);
-    if (!plain) up(s.rule_vals, (int64_t)b * SVL_RULES_BIASES * 4, vals.data(), SVL_RULES_BIASES * 4);
-    up(s.rule_rows, b * 4ll, &row, 4);
-    if (row >= 0) up(s.rule_masks, b * words * 4, rules->allowed, words * 4);
-    check_cuda(cudaStreamSynchronize(st), "rules");  // the host values above live until here
+  auto up = [&](DevBuf& to, const auto& from, int64_t per_stream) {
+    if (!from.empty())
+      check_cuda(cudaMemcpyAsync(to.as<uint8_t>() + lo * per_stream * 4, from.data(), from.size() * 4, cudaMemcpyHostToDevice, st), "upload");
   };
-  for (int b = 0; b < B; b++) {
-    if (stream < 0 || b == stream)
-      put(b, false);
-    else if (!s.rules)
-      put(b, true);
+  up(s.rule_rep, rep, 1);
+  up(s.rule_freq, freq, 1);
+  up(s.rule_pres, pres, 1);
+  up(s.rule_ids, ids, SVL_RULES_BIASES);
+  up(s.rule_vals, vals, SVL_RULES_BIASES);
+  up(s.rule_rows, rows, 1);
+  up(s.rule_masks, masks, words);
+  check_cuda(cudaStreamSynchronize(st), "rules");  // the host values above live until here
+  // The captured steps read the rules from these buffers, but for first_penalised, a kernel argument: they
+  // are captured again only where the rules first come or it changes (a grammar's next set of tokens before
+  // each step of an STT-1b stream, update and step: 1,099 us with a capture, 663 without; the step alone 614).
+  if (first_time || (rules && rules->first_penalised != s.rules_first)) {
+    for (auto& kv : s.graphs) cudaGraphExecDestroy(kv.second);
+    s.graphs.clear();
+    s.graph_kernels.clear();
   }
   if (rules) s.rules_first = rules->first_penalised;
-  // The captured steps do not have the rules (or have the old first_penalised).
-  for (auto& kv : s.graphs) cudaGraphExecDestroy(kv.second);
-  s.graphs.clear();
-  s.graph_kernels.clear();
   s.rules = true;
 }
 
