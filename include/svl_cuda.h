@@ -229,9 +229,14 @@ typedef struct svl_stt_rules {
   const uint32_t* allowed; /* bit v % 32 of word v / 32: token v may follow; NULL = every token */
 } svl_stt_rules;
 /* The logits that a step returns are those after the rules. A step that no token may follow
- * yields token 0xFFFFFFFF, which the next step refuses as out of range. first_penalised is the
- * state's: the last call's value holds for every stream. A reset stream's recorded tokens are
- * forgotten, svl_state_copy copies them between states that both have rules. */
+ * yields token 0xFFFFFFFF for that stream, which as a step's input is out of range: svl_stt_step
+ * refuses it before anything runs (the caller may give that stream another token);
+ * svl_stt_run_frames, which feeds it back on the device, returns SVL_ERR_INVALID_INPUT after its
+ * last frame, with every frame's tokens and the rings moved on; svl_stt_step_device cannot
+ * refuse: the stream goes on as if it had said token 0, and svl_state_error reports it.
+ * first_penalised is the state's: the last call's value holds for every stream, and a new value has
+ * the steps captured again. A reset stream's recorded tokens are forgotten, svl_state_copy copies
+ * them between states that both have rules. */
 SVL_API svl_status svl_state_set_rules(svl_state* state, int32_t stream, const svl_stt_rules* rules);
 
 /* Transformer::forward (nn/transformer.rs:139-154) of one stream over xs [t][d_model] (host,

@@ -125,6 +125,11 @@ class State:
         """No rules for one stream, or for all."""
         _lib.check(_lib.lib().svl_state_set_rules(self.handle, stream, None))
 
+    def check(self):
+        """Waits for the device; raises if a device-side step since the last check met a token out of range (one
+        that a grammar without a way on left is 0xFFFFFFFF) or a bounded wait that ran out (svl_state_error)."""
+        _lib.check(_lib.lib().svl_state_error(self.handle))
+
     def save_voice(self, path, stream: int = 0):
         """Voice::save (tts/voice.rs:78-99): this stream's KV state as a safetensors voice."""
         _lib.check(_lib.lib().svl_voice_save(self.handle, stream, str(path).encode()))

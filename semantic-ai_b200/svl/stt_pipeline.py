@@ -34,7 +34,10 @@ class SttPipeline:
     def step(self, pcm):
         """pcm: CUDA float32 [streams][channels][frame_size], one frame per stream. Returns the
         frame's text tokens and audio codes as CUDA int32 tensors ([streams], [streams][n_q]),
-        valid on this pipeline's stream (synchronise it, or wait on it, before reading)."""
+        valid on this pipeline's stream (synchronise it, or wait on it, before reading).
+
+        A stream whose grammar (lm_state.set_rules) allows no token gets -1 and goes on as if it had said token
+        0: steps do not wait, so only check() raises."""
         import torch
         s = self.stream
         s.wait_stream(torch.cuda.current_stream())
@@ -50,3 +53,8 @@ class SttPipeline:
         self.text = out
         self.steps += 1
         return out, codes
+
+    def check(self):
+        """Waits for the device; raises if a step since the last check was fed a token out of range, as after a
+        grammar that left none, or if a bounded wait ran out."""
+        self.lm_state.check()

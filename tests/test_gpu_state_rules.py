@@ -5,7 +5,9 @@ import time
 import numpy as np
 import pytest
 
-from svl import LanguageModel, config, synth
+from svl import LanguageModel, codec, config, synth
+from svl._lib import SvlError
+from svl.stt_pipeline import SttPipeline
 from test_gpu_f8_model import check_rules
 
 pytestmark = pytest.mark.gpu
@@ -59,3 +61,52 @@ def test_rules_keep_the_captured_step(svl_lib):
     captured = median(lambda i: dict(first_penalised=4 + i % 2))
     print(f"step {step * 1e6:.0f} us, with new rules {kept * 1e6:.0f}, captured again {captured * 1e6:.0f}")
     assert kept - step < 0.4 * (captured - step)
+
+
+def test_pipeline_with_no_token_left(svl_lib):
+    """A grammar that allows nothing: -1 for its stream, told by check() after the step that was fed it, and by no
+    other; the other stream's tokens are those of a pipeline without rules."""
+    import torch
+    stt = config.stt_toy(card=2048, n_q=32)
+    mcfg = codec.stt_mimi(codec.ENCODER)
+    w = synth.mimi_weights(mcfg)
+    w.update(synth.rvq_weights(32, 2048))
+    cfg = stt.transformer("f32", "f32")
+    mimi, q, lm = codec.Mimi(mcfg, w), codec.Quantizer(32, 2048, w), LanguageModel(stt, cfg, synth.stt_weights(stt, cfg))
+    plain, ruled = SttPipeline(mimi, q, lm, 2), SttPipeline(mimi, q, lm, 2)
+    ruled.lm_state.set_rules(stream=0, allowed=[])
+    pcm = torch.from_numpy((0.3 * np.random.default_rng(1).standard_normal((4, 2, 1, mimi.frame_size))).astype(np.float32)).cuda()
+    tokens = []
+    for f in range(4):
+        want, got = plain.step(pcm[f])[0], ruled.step(pcm[f])[0]
+        torch.cuda.synchronize()
+        tokens.append(got[0].item())
+        assert got[1] == want[1]
+        if f == 0:
+            ruled.check()
+        elif f == 1:
+            with pytest.raises(SvlError, match="token"):
+                ruled.check()
+            ruled.check()
+            ruled.lm_state.clear_rules(0)
+    # Step 2 was still fed the -1 of step 1.
+    assert tokens[:2] == [-1, -1] and tokens[2] >= 0 and tokens[3] >= 0
+    with pytest.raises(SvlError, match="token"):
+        ruled.check()
+    plain.check()
+
+
+def test_run_frames_with_no_token_left(svl_lib):
+    """run_frames raises after its last frame; lm.step goes on with another token for that stream."""
+    stt, gm = toy()
+    st = gm.init_state(2)
+    st.set_rules(stream=1, allowed=[])
+    audio = synth.audio_tokens(stt, 4, streams=2)
+    with pytest.raises(SvlError, match="token"):
+        gm.run_frames(audio, st)
+    assert [st.position(b) for b in range(2)] == [4, 4]
+    with pytest.raises(SvlError, match="token"):
+        gm.step([1, 0xFFFFFFFF], audio[0], st)
+    assert st.position(0) == 4
+    st.clear_rules(1)
+    assert all(t < stt.text_card for t in gm.step([1, 2], audio[0], st))
