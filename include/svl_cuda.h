@@ -420,7 +420,7 @@ SVL_API svl_status svl_rvq_encode_device(svl_rvq* rvq, int32_t batch, int32_t fr
  *   d_sum may be d_x or d_residual itself (same pointer and stride).
  *   norm_kind: SVL_NORM_RMS (h / sqrt(mean(h^2) + eps) * weight), SVL_NORM_LAYER
  *   ((h - mean) / sqrt(var + eps) * weight + bias) or -1 (y = h); d_weight and d_bias are f32
- *   [k], NULL = ones and zeros.
+ *   [k], NULL = ones and zeros; SVL_ERR_INVALID_INPUT where the norm has no place for them.
  *   Per block: a = max(max |y|, 2^-100), scale = a / 448, q = e4m3(y * 448 / a), to nearest even.
  *   Without a norm the quotient is rounded once before (to f32), so that a y of few bits, as in bf16
  *   rows, gets the nearest e4m3 value; with one, 448 / a and the product are rounded. A block that

@@ -589,6 +589,8 @@ SVL_API svl_status svl_add_norm_f8_device(int32_t device, int64_t rows, int32_t 
     require(eps >= 0.f, "eps must not be negative");
     svl::require_aligned(dtype == SVL_DT_F32 ? 4 : 2, d_x, d_residual, d_sum);
     svl::require_aligned(4, d_weight, d_bias, d_scales);
+    require(!d_weight || norm_kind >= 0, "d_weight without a norm");
+    require(!d_bias || norm_kind == SVL_NORM_LAYER, "d_bias needs the layer norm");
     OnDevice on(device);
     svl::NormF8Params p{};
     p.x = d_x;

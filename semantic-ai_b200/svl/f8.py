@@ -23,7 +23,8 @@ def add_norm_f8(x, residual=None, norm: str | None = "rms", weight=None, bias=No
                 out_sum=None, stream=None):
     """h = x + residual, y = norm(h) ("rms", "layer" or None: y = h), y as e4m3 rows.
 
-    x and residual: CUDA [rows, k], float32 or bfloat16; weight and bias: float32 [k] or None.
+    x and residual: CUDA [rows, k], float32 or bfloat16; weight (of a norm) and bias (of the layer norm):
+    float32 [k] or None.
     Returns (q, scales, h): q float8_e4m3fn [rows, k] (rows 16-byte aligned), scales float32
     [ceil(k / 128), rows], and the sum h in x's dtype: out_sum if given (it may be x or residual),
     a new tensor with a residual, x itself without. out_sum must not overlap x or residual otherwise."""

@@ -127,3 +127,12 @@ def test_linear_create_refuses_misaligned(svl_lib):
     for s, b in ((PTR + 2, None), (PTR, PTR + 1)):
         assert svl_lib.svl_f8_linear_create_device(128, 128, PTR, 128, s, b, 0, None, ctypes.byref(h)) == INVALID
         assert b"aligned" in svl_lib.svl_last_error()
+
+
+@pytest.mark.parametrize("change,message", [(dict(b=PTR), b"bias"), (dict(norm=-1, b=PTR), b"bias"), (dict(norm=-1, w=PTR), b"weight"),
+                                            (dict(norm=-1, w=PTR, b=PTR), b"weight")])
+def test_norm_refuses_what_it_would_leave_out(svl_lib, change, message):
+    """A weight without a norm, a bias of a norm that adds none."""
+    assert norm(svl_lib, **change) == INVALID
+    assert message in svl_lib.svl_last_error()
+    assert norm(svl_lib, rows=0, **change) == 0
