@@ -22,9 +22,14 @@ ops.bind(_address("svl_add_norm_f8_device"), _address("svl_f8_linear_device"), _
          _address("svl_last_error"), _lib.SvlError)
 
 
+def of(stream, device):
+    """`stream`, refused if it is not one of the tensors' device."""
+    if stream.device != device:
+        raise ValueError(f"stream must be one of {device}: got one of {stream.device}")
+    return stream
+
+
 def on(stream, device):
     """The context in which a call runs and allocates on `stream`, a stream of the tensors' device.
     (Outputs that belonged to another stream could be given out again while `stream` still writes.)"""
-    if stream.device != device:
-        raise ValueError(f"stream must be one of {device}: got one of {stream.device}")
-    return torch.cuda.stream(stream)
+    return torch.cuda.stream(of(stream, device))

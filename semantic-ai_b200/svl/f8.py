@@ -12,7 +12,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._ops import on, ops
+from ._ops import of, on, ops
 from .model import tensor_views
 
 BLOCK = 128
@@ -39,8 +39,9 @@ class F8Linear:
     """An e4m3 matrix [n][k] with f32 scales per 128 x 128 block, and an optional bias.
 
     weight: float8_e4m3fn CUDA [n, k], scales: float32 CUDA [ceil(n / 128), ceil(k / 128)], bias:
-    float32 CUDA [n] or None; all are copied. F8Linear.quantise() makes one from f32 weights. It has to
-    outlive the CUDA graphs that captured its products."""
+    float32 CUDA [n] or None; all are copied, after the work on torch's current stream of their device (or on
+    `stream`), which the call waits for. F8Linear.quantise() makes one from f32 weights. It has to outlive the
+    CUDA graphs that captured its products."""
 
     handle = None
 
@@ -56,7 +57,7 @@ class F8Linear:
             if t is not None and (tuple(t.shape) != shape or t.dtype != torch.float32 or not t.is_contiguous() or t.device != device):
                 raise ValueError(f"{name} must be contiguous float32 {shape} on {device}: got {tuple(t.shape)}, {t.dtype}, {t.device}")
         h = ctypes.c_void_p()
-        s = torch.cuda.current_stream(device) if stream is None else stream
+        s = torch.cuda.current_stream(device) if stream is None else of(stream, device)
         _lib.check(_lib.lib().svl_f8_linear_create_device(
             n, k, weight.data_ptr(), weight.stride(0) if n > 1 else max(weight.stride(0), k), scales.data_ptr(),
             None if bias is None else bias.data_ptr(), device.index, s.cuda_stream, ctypes.byref(h)))

@@ -64,3 +64,18 @@ def test_weights_of_few_bits_take_the_nearest(svl_lib):
             blk = w[i:i + 128, j:j + 128].astype(np.float64)
             top = np.abs(blk).max()
             np.testing.assert_array_equal(got[i:i + 128, j:j + 128], nearest_e4m3(blk * 448 / top).astype(F) * F(F(top) / F(448)))
+
+
+def test_matrix_refuses_a_stream_of_another_device(svl_lib):
+    """As the operators do: the copies would not wait for the work of the stream that was meant."""
+    import types
+
+    import torch
+
+    import svl
+    w, s = torch.zeros(128, 128, device="cuda").to(torch.float8_e4m3fn), torch.ones(1, 1, device="cuda")
+    # What a stream of a second GPU looks like, its default one.
+    elsewhere = types.SimpleNamespace(device=torch.device("cuda", torch.cuda.current_device() + 1), cuda_stream=0)
+    with pytest.raises(ValueError, match="stream must be one of"):
+        svl.F8Linear(w, s, stream=elsewhere)
+    svl.F8Linear(w, s, stream=torch.cuda.Stream()).close()
