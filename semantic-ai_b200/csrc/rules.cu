@@ -475,6 +475,22 @@ int64_t clusters_at_once(int n) {
   return c;
 }
 
+// A CTA's part of a row: its range of the vocabulary, taken in chunks, and the shared memory of their lists.
+struct Part {
+  int range, chunk, slots;
+  bool direct;
+  size_t smem;
+  Part(int64_t span, int split, int entries) {
+    range = (int)((span + split - 1) / split + 31) / 32 * 32;
+    chunk = std::min(range, entries > kLongLists ? kMaxChunkLong : kMaxChunk);
+    direct = chunk <= kDirect;
+    slots = direct ? chunk : std::min(entries, chunk);
+    smem = entries ? (size_t)chunk / 4 + (size_t)slots * kSlotBytes : 0;
+  }
+  // CTAs that an SM's 228 KB hold, each with 1 KB of its own and less than 1 KB of static shared memory.
+  int per_sm() const { return (int)(228 * 1024 / (smem + 2048)); }
+};
+
 // CTAs per row. One where it has at most 16,384 tokens to go through: a cluster costs more than its
 // share of the work saves. Up to 148 rows: the most that still run at once with an SM each (16
 // rows of 131,072 bf16 tokens without rules: 6 CTAs 4.3 us, 8 in two waves 7.4; 64 rows: 2 CTAs
@@ -482,19 +498,21 @@ int64_t clusters_at_once(int n) {
 // at once (120 rows of 50,257 f32 tokens, a history of 500: 25 us with one, 20 with two). More rows: the number whose waves take the shortest, the lists and the
 // joining of a CTA's results counted like 12,000 tokens (192 rows of 131,072 bf16 tokens with all
 // rules: 5 CTAs 52 us, 2 CTAs 54, 8 CTAs 59, 1 CTA 85; 512 rows of 32,000: 1 CTA 11.3, 2 CTAs 14.3).
+// Long lists leave room for fewer CTAs on an SM than the kernel's registers do.
 template <class T>
-int rules_split(int64_t rows, int64_t span, bool lists) {
+int rules_split(int64_t rows, int64_t span, int entries) {
   if (span <= 16384) return 1;
   int split = 1;
   if (rows <= 148) {
     for (int n = 2; n <= 8; n++)
       if (rows <= clusters_at_once<rules_kernel<T, 512, 1>, 512, 1>(n)) split = n;
-    if (split == 1 && lists && rows <= clusters_at_once<rules_kernel<T, 512, 2>, 512, 2>(2)) split = 2;
+    if (split == 1 && entries && Part(span, 2, entries).per_sm() >= 2 && rows <= clusters_at_once<rules_kernel<T, 512, 2>, 512, 2>(2)) split = 2;
     return split;
   }
   int64_t least = INT64_MAX;
   for (int n = 1; n <= 8; n++) {
-    const int64_t at_once = clusters_at_once<rules_kernel<T, 256, 4>, 256, 4>(n);
+    const int fit = std::min(4, Part(span, n, entries).per_sm());
+    const int64_t at_once = std::max<int64_t>(1, clusters_at_once<rules_kernel<T, 256, 4>, 256, 4>(n) * fit / 4);
     const int64_t t = (rows + at_once - 1) / at_once * (span / n + 12000);
     if (t < least) {
       least = t;
@@ -510,21 +528,17 @@ void launch_rules(const RulesParams& p, cudaStream_t s) {
   const int64_t span = (int64_t)p.vocab + ve - 1;  // with the lead of the worst row
   const int entries = (p.rules.d_history ? p.rules.history_cap : 0) + (p.rules.d_bias_ids ? p.rules.bias_cap : 0);
   const int split = p.bf16 ? rules_split<__nv_bfloat16>(p.rows, span, entries) : rules_split<float>(p.rows, span, entries);
-  const int range = (int)((span + split - 1) / split + 31) / 32 * 32;
-  const int chunk = std::min(range, entries > kLongLists ? kMaxChunkLong : kMaxChunk);
+  const Part part(span, split, entries);
   // Two pieces per thread; 512 threads where two CTAs per SM take all rows (256 rows of 4,001 f32
   // tokens with all rules: 10 us, 13 with 256 threads).
   const int64_t ctas = p.rows * split;
   const int most = ctas <= 2 * 148 ? 512 : 256;
-  const int threads = std::min(most, std::max(64, ((chunk + 2 * ve - 1) / (2 * ve) + 31) / 32 * 32));
-  const int direct = chunk <= kDirect;
-  const int slots = direct ? chunk : std::min(entries, chunk);
-  const size_t smem = entries ? (size_t)chunk / 4 + (size_t)slots * kSlotBytes : 0;
+  const int threads = std::min(most, std::max(64, ((part.chunk + 2 * ve - 1) / (2 * ve) + 31) / 32 * 32));
   auto launch = [&](auto kernel) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.rows * split));
   cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = part.smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -535,16 +549,16 @@ void launch_rules(const RulesParams& p, cudaStream_t s) {
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = split > 1 ? 2 : 1;
-  check_cuda(cudaLaunchKernelEx(&cfg, kernel, p, split, range, chunk, slots, direct), "rules launch");
+  check_cuda(cudaLaunchKernelEx(&cfg, kernel, p, split, part.range, part.chunk, part.slots, (int)part.direct), "rules launch");
   };
   auto variant = [&](auto type) {
     using T = decltype(type);
     if (ctas <= 148)
-      launch(with_smem<rules_kernel<T, 512, 1>>(smem));
+      launch(with_smem<rules_kernel<T, 512, 1>>(part.smem));
     else if (ctas <= 2 * 148)
-      launch(with_smem<rules_kernel<T, 512, 2>>(smem));
+      launch(with_smem<rules_kernel<T, 512, 2>>(part.smem));
     else
-      launch(with_smem<rules_kernel<T, 256, 4>>(smem));
+      launch(with_smem<rules_kernel<T, 256, 4>>(part.smem));
   };
   p.bf16 ? variant(__nv_bfloat16()) : variant(float());
 }

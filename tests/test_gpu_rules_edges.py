@@ -43,6 +43,21 @@ def test_repeated_biases(svl_lib, rows, vocab, entries, history, pattern):
     check(logits, r, "bf16", offset=3, in_place=True)
 
 
+def shortest(call):
+    """Device time of a call, ms: the shortest of some runs of ten."""
+    import torch
+    best = 1e9
+    for _ in range(6):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        for _ in range(10):
+            call()
+        b.record()
+        torch.cuda.synchronize()
+        best = min(best, a.elapsed_time(b) / 10)
+    return best
+
+
 @pytest.mark.parametrize("rows,vocab,entries", [(1, 131072, 16384), (64, 32000, 4096)])
 def test_a_repeated_id_costs_no_more_than_the_list(svl_lib, rows, vocab, entries):
     """The time grows with the list, not with its square, when an id stands there twice: one more pass over the
@@ -59,18 +74,30 @@ def test_a_repeated_id_costs_no_more_than_the_list(svl_lib, rows, vocab, entries
 
     def time(ids):
         ids = torch.from_numpy(ids).cuda()
-        call = lambda: svl.logits_rules(logits, bias_ids=ids, bias_values=values)  # noqa: E731
-        best = 1e9
-        for _ in range(6):
-            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
-            a.record()
-            for _ in range(5):
-                call()
-            b.record()
-            torch.cuda.synchronize()
-            best = min(best, a.elapsed_time(b) / 5)
-        return best
+        return shortest(lambda: svl.logits_rules(logits, bias_ids=ids, bias_values=values))
 
     plain, repeated = time(once), time(twice)
     print(f"{rows} x {vocab}, {entries} biases: {plain * 1e3:.1f} us, {repeated * 1e3:.1f} with an id twice")
     assert repeated < 8 * plain
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_long_lists_leave_room_for_fewer_rows_at_once(svl_lib, dtype):
+    """Rows are shared among CTAs by how many run at once with the shared memory that their lists take: twice the
+    rows take no more than about twice the time. (2.9 times f32, 2.5 bf16, where the plan left the lists out.)"""
+    import torch
+
+    import svl
+    t = {"f32": torch.float32, "bf16": torch.bfloat16}[dtype]
+    vocab, said = 50257, 6000
+    g = torch.Generator(device="cuda").manual_seed(2)
+    logits = torch.randn(256, vocab, device="cuda", generator=g).to(t)
+    history = torch.randint(0, vocab, (256, said), device="cuda", dtype=torch.int32, generator=g)
+    lengths, penalty = torch.full((256,), said, dtype=torch.int32, device="cuda"), torch.full((256,), 1.5, device="cuda")
+    rules = lambda n: svl.logits_rules(logits[:n], history=history[:n], lengths=lengths[:n], repetition=penalty[:n])  # noqa: E731
+    half, all_ = shortest(lambda: rules(128)), shortest(lambda: rules(256))
+    print(f"{dtype}: 128 rows {half * 1e3:.1f} us, 256 rows {all_ * 1e3:.1f}")
+    assert all_ < 2.1 * half
+    want, token = rules(128)
+    got, tokens = rules(256)
+    assert torch.equal(got[:128], want) and torch.equal(tokens[:128], token)
