@@ -54,9 +54,24 @@ def _compile(src: Path, extra: list[str]) -> Path:
     return obj
 
 
+def _built_for() -> str | None:
+    """What the binding has to match besides its sources: torch, its C++ ABI and Python's. None without torch."""
+    import sysconfig
+
+    try:
+        import torch
+    except ImportError:
+        return None
+    return f"torch {torch.__version__} cxx11 {int(torch._C._GLIBCXX_USE_CXX11_ABI)} {sysconfig.get_config_var('EXT_SUFFIX')}"
+
+
 def _build_torch_ops() -> None:
+    key, stamp = _built_for(), OUT / "torch_ops.stamp"
+    if key is None:
+        sys.stderr.write(f"{TORCH_OPS.name} is not built: torch cannot be imported\n")
+        return
     newest = max(TORCH_SRC.stat().st_mtime, (PKG.parent / "include" / "svl_cuda.h").stat().st_mtime)
-    if TORCH_OPS.exists() and TORCH_OPS.stat().st_mtime >= newest:
+    if TORCH_OPS.exists() and TORCH_OPS.stat().st_mtime >= newest and stamp.exists() and stamp.read_text() == key:
         return
     import sysconfig
 
@@ -72,17 +87,24 @@ def _build_torch_ops() -> None:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"building {TORCH_OPS.name} failed:\n{r.stdout}\n{r.stderr}")
+    stamp.write_text(key)
 
 
 def build(verbose: bool = False, extra: list[str] | None = None) -> Path:
+    """The library and, where torch can be imported, the binding, whose failure leaves the library built."""
     OUT.mkdir(exist_ok=True)
     extra = extra or []
     with cf.ThreadPoolExecutor(max_workers=os.cpu_count() or 4) as ex:
         ops = ex.submit(_build_torch_ops)
         objs = list(ex.map(lambda s: _compile(s, extra), _sources()))
-        ops.result()
+    _link(objs, verbose)
+    ops.result()
+    return LIB
+
+
+def _link(objs: list[Path], verbose: bool) -> None:
     if LIB.exists() and LIB.stat().st_mtime >= max(o.stat().st_mtime for o in objs):
-        return LIB
+        return
     cmd = [NVCC, "-shared", "-gencode", "arch=compute_100a,code=sm_100a",
            "-Xcompiler", "-fPIC", "-o", str(LIB), *map(str, objs), "-cudart", "static"]
     r = subprocess.run(cmd, capture_output=True, text=True)
@@ -90,7 +112,6 @@ def build(verbose: bool = False, extra: list[str] | None = None) -> Path:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     if verbose:
         print(f"built {LIB}")
-    return LIB
 
 
 if __name__ == "__main__":
