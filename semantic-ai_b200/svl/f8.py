@@ -93,6 +93,10 @@ class F8Linear:
                 return self(q, scales, out_dtype, out)
         return ops.f8_linear(self.handle, self.n, self.k, self.device, q, scales, out_dtype, out)
 
+    def __reduce_ex__(self, protocol):
+        # A copy would own the same matrix, and both would free it.
+        raise TypeError("an F8Linear cannot be copied or pickled")
+
     def check(self):
         """Waits for the device; raises if a bounded device-side wait of a product ran out."""
         _lib.check(_lib.lib().svl_f8_linear_error(self.handle))

@@ -136,3 +136,15 @@ def test_norm_refuses_what_it_would_leave_out(svl_lib, change, message):
     assert norm(svl_lib, **change) == INVALID
     assert message in svl_lib.svl_last_error()
     assert norm(svl_lib, rows=0, **change) == 0
+
+
+def test_linear_refuses_copies():
+    """Two handles of one matrix would free it twice."""
+    import copy
+    import pickle
+
+    import svl
+    lin = svl.F8Linear.__new__(svl.F8Linear)  # no matrix: it is the copy that is refused
+    for make in (copy.copy, copy.deepcopy, pickle.dumps, lambda x: copy.deepcopy({"head": x})):
+        with pytest.raises(TypeError, match="cannot be copied"):
+            make(lin)
