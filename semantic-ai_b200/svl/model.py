@@ -104,12 +104,14 @@ class State:
         bits = None
         if allowed is not None:
             card = self.model.stt.text_card
-            a = np.asarray(allowed)
+            a = np.asarray(sorted(allowed) if isinstance(allowed, (set, frozenset)) else allowed)
             if a.dtype == bool:
                 if a.shape != (card,):
                     raise ValueError(f"allowed must have {card} truth values: got {a.shape}")
                 ok = a
             else:
+                if a.size and not np.issubdtype(a.dtype, np.integer):
+                    raise ValueError(f"allowed must be token ids or truth values: got {a.dtype}")
                 if a.size and (a.min() < 0 or a.max() >= card):
                     raise ValueError(f"allowed tokens must be below {card}")
                 ok = np.zeros(card, bool)

@@ -148,3 +148,36 @@ def test_linear_refuses_copies():
     for make in (copy.copy, copy.deepcopy, pickle.dumps, lambda x: copy.deepcopy({"head": x})):
         with pytest.raises(TypeError, match="cannot be copied"):
             make(lin)
+
+
+@pytest.fixture
+def set_rules(monkeypatch):
+    """State.set_rules on a library that only records what it is given: the mask's allowed tokens."""
+    import types
+
+    import numpy as np
+
+    from svl import _lib, model
+    given = []
+
+    def record(handle, stream, rules):
+        r = ctypes.cast(rules, ctypes.POINTER(model.CSttRules)).contents
+        words = np.array([r.allowed[i] for i in range(4)], np.uint32)
+        given.append(np.flatnonzero(np.unpackbits(words.view(np.uint8), bitorder="little")).tolist())
+        return 0
+
+    monkeypatch.setattr(_lib, "lib", lambda: types.SimpleNamespace(svl_state_set_rules=record))
+    state = model.State.__new__(model.State)
+    state.handle, state.model = None, types.SimpleNamespace(stt=types.SimpleNamespace(text_card=100))
+    return lambda allowed: (state.set_rules(allowed=allowed), given[-1])[1]
+
+
+def test_allowed_tokens(set_rules):
+    import numpy as np
+    for allowed in ([5, 7, 99], (99, 5, 7), {5, 7, 99}, frozenset({5, 7, 99}), np.array([5, 7, 99], np.int16), [i in (5, 7, 99) for i in range(100)]):
+        assert set_rules(allowed) == [5, 7, 99]
+    assert set_rules([]) == set_rules(set()) == []
+    assert set_rules(range(4, 40)) == list(range(4, 40))
+    for wrong in ([1.5], [5.0, 7.0], [float("nan")], ["5"], [None], [-1], [100], [True] * 99):
+        with pytest.raises(ValueError, match="allowed"):
+            set_rules(wrong)
