@@ -92,7 +92,7 @@ __device__ __forceinline__ Raw<T, V> pack(const float (&v)[V]) {
 // Rows that start anywhere. A thread's V values are read in the aligned 16-byte pieces that hold at
 // least one of them (one more than V values take), as they come; `shifted` then cuts the values
 // out. (Value by value, every load of a warp would touch a sector per lane: 16,384
-// x 2,561 with a residual bf16 took 254 us, 115 this way.)
+// x 2,561 with a residual bf16 took 254 us, 111 this way.)
 template <class T, int V>
 struct RawOdd {
   uint4 v[V * sizeof(T) / 16 + 1];
@@ -226,6 +226,8 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
 //
 // Measured with a residual: 16,384 x 2,560 bf16 48 us (6.2 TB/s; 59 with loads of 16 bytes, which made
 // L1 the bound), 8,192 x 2,048 f32 35 us (6.2 TB/s); 512 x 1,024 layer norm f32 3.8 us; 1 x 2,048 2.1 us.
+// Rows of four pieces have up to 1,024 threads and so 64 registers, of which f32 ones spill 212 bytes and
+// bf16 ones 164: 4,096 x 10,240 f32 123 us (4.4 TB/s), 2,048 x 20,000 bf16 91 us (3.1 TB/s).
 //
 // The compiler's choice of registers is left to it but for bf16 rows of one piece. For odd ones it would
 // take too few (16,384 x 727: 47 us, 38.5 with all that one CTA may have; aligned rows: 28); for
@@ -246,7 +248,8 @@ __global__ void __launch_bounds__(I == 4 ? 1024 : 512, kLeastCtas<T, I, Odd>) no
   const bool ww = reinterpret_cast<uintptr_t>(p.weight) % 32 == 0, bw = reinterpret_cast<uintptr_t>(p.bias) % 32 == 0;
   auto on32 = [](const void* base, int64_t stride) { return (reinterpret_cast<uintptr_t>(base) | (uint64_t)stride * sizeof(T)) % 32 == 0; };
   const bool x32 = on32(p.x, p.x_stride), r32 = on32(p.residual, p.residual_stride), s32 = on32(p.sum, p.sum_stride);
-  constexpr bool kShift = Odd && I < 4;  // the longest rows leave no registers for it: 4,096 x 10,241 f32 56 us, 70 with
+  // The longest rows leave few registers for it: 4,096 x 10,241 f32 54 us, 65 with; though with a residual 247, 198 with.
+  constexpr bool kShift = Odd && I < 4;
   using Piece = typename std::conditional<kShift, RawOdd<T, V>, Raw<T, V>>::type;
   Piece nx[I], nr[I];
   auto load = [&](const void* base, int64_t at, int have, bool wider) {

@@ -719,7 +719,8 @@ __global__ void __launch_bounds__(Wide::kThreads, 1) f8_wide_kernel(const __grid
 // ---- very many rows: 128 x 256 tiles ---------------------------------------------------------------
 
 // The same with 256 matrix rows per tile (48 KB of operands per block for the work that takes 64 KB
-// as two tiles of 128: with the narrower tiles the operands' way from L2 is the bound). Scaling and
+// as two tiles of 128: with the narrower tiles the operands' way from L2 is the bound). The 20 warps leave a
+// thread 96 registers, 64 of which hold its sums; the compiler spills 92 bytes. Scaling and
 // adding a block's 128 x 256 products takes the SM's FMA pipes 256 clocks of the 512 that the
 // products take, so it is spread over 16 warps, four per scheduler, each with 64 columns of 32
 // rows. A warp of its own fetches the rows' scales into shared memory, 8 blocks at a time.
@@ -1010,8 +1011,11 @@ void launch_big(F8Args a, cudaStream_t s) {
 // Which kernel. Up to 32 rows the matrix rows as M; above too, in tiles of 32 rows, as long as all of
 // them run at once and have no more than 2,112 blocks in all, two of which an SM loads about as
 // fast as one of a 128 x 128 tile, but whose tiles start, end and share a long axis faster: 147 x
-// 225 x 2048 4.3 us against 6.9, 128 x 1024 x 5632 (1,408 blocks) 6.7 against 8.7, 256 x 2048 x 2048
-// (2,048 blocks) 8.0 both, 128 x 2048 x 5632 (2,816 blocks) 9.4 against 9.0. Else 128 x 128 tiles or
+// 225 x 2048 4.4 us against 7.1, 128 x 1024 x 5632 (1,408 blocks) 6.8 against 8.7, 160 x 1024 x 5632
+// (1,760) 8.0 against 8.7, 128 x 2048 x 5120 (2,560) 9.0 against 8.5, 128 x 2048 x 5632 (2,816) 9.7
+// against 8.9. From 2,048 blocks (8.2 against 7.9 in 128 tiles) to 2,304 (8.6 against 8.2) the two are
+// within 5 % of each other, either way (2,112 in 48 tiles: 8.3 against 8.7), and the border lies there.
+// Else 128 x 128 tiles or
 // 128 x 256: a wave of the larger ones takes 1.55 times as long (1024 x 11264 x 2048: 35 us in 5
 // waves, 33 in 3; 512 x 11264 x 2048: 22 us in 3, 23 in 2; 256 x 11264 x 2048: 15.5 us in 2, 13.3 in 1).
 void launch_f8_gemm(const F8GemmParams& p, cudaStream_t s) {

@@ -123,13 +123,14 @@ __device__ __forceinline__ void add_repeated(const int32_t* ids, const float* va
 // logits are fetched before the stream, which passes over them as it does over tokens that the
 // grammar forbids, and written after it. The row's first logits and list entries are on their way
 // meanwhile. A chunk of at most 8,192 tokens has a count and an entry for each (`direct`): zeroing them
-// takes less than giving slots (256 rows of 4,001 f32 tokens with all rules: 10.4 us, 11.3 with
+// takes less than giving slots (256 rows of 4,001 f32 tokens with all rules: 9.0 us, 9.9 with
 // slots).
 //
-// Measured: 1 row of 8,000 f32 tokens with a history of 250, 16 biases and a mask 5.6 us (2.8 without
-// rules); 256 rows of 4,001 f32 with all rules 8.9 us; 192 rows of 131,072 bf16 with all rules, a
-// history of 2,048 each, 49.5 us (2.1 TB/s), 21 without any rule. More warps per SM would hide
-// more of the lists' latency, but below 64 registers the spills cost more than they bring.
+// Measured: 1 row of 8,000 f32 tokens with a history of 250, 16 biases and a mask 5.7 us (2.9 without
+// rules); 256 rows of 4,001 f32 with all rules 9.0 us; 192 rows of 131,072 bf16 with all rules, a
+// history of 2,048 each, 50.4 us (2.1 TB/s), 21 without any rule. More warps per SM would hide
+// more of the lists' latency, but below 64 registers, at which the kernels of two and more CTAs per
+// SM already spill up to 36 bytes, the spills cost more than they bring.
 //
 // Positions are counted from the 16-byte boundary at or before the row's start ("lead" elements
 // before it), so that every row is read in aligned 16-byte pieces, also where rows of an odd
@@ -493,12 +494,14 @@ struct Part {
 
 // CTAs per row. One where it has at most 16,384 tokens to go through: a cluster costs more than its
 // share of the work saves. Up to 148 rows: the most that still run at once with an SM each (16
-// rows of 131,072 bf16 tokens without rules: 6 CTAs 4.3 us, 8 in two waves 7.4; 64 rows: 2 CTAs
-// 7.2, 8 CTAs 8.3). Where that is one CTA, two of a half each per SM for rows with lists, if they run
-// at once (120 rows of 50,257 f32 tokens, a history of 500: 25 us with one, 20 with two). More rows: the number whose waves take the shortest, the lists and the
+// rows of 131,072 bf16 tokens without rules: 6 CTAs 4.2 us, 8 in two waves 7.3; 64 rows: 2 CTAs
+// 7.0, 8 CTAs 8.5). Where that is one CTA, two of a half each per SM for rows with lists, if they run
+// at once (120 rows of 50,257 f32 tokens, a history of 500: 26 us with one, 21 with two). More
+// rows: the number whose waves take the shortest, the lists and the
 // joining of a CTA's results counted like 12,000 tokens (192 rows of 131,072 bf16 tokens with all
-// rules: 5 CTAs 52 us, 2 CTAs 54, 8 CTAs 59, 1 CTA 85; 512 rows of 32,000: 1 CTA 11.3, 2 CTAs 14.3).
-// Long lists leave room for fewer CTAs on an SM than the kernel's registers do.
+// rules: 5 CTAs 50.3 us, 2 CTAs 53, 8 CTAs 57, 1 CTA, of 512 threads then, 47; 512 rows of 32,000: 1 CTA 33, 2
+// CTAs 41). Long lists leave room for fewer CTAs on an SM than the kernel's registers do, which counts (256 rows
+// of 50,257 bf16 tokens with a history of 6,000: 31 us, 56 as if the lists took no memory).
 template <class T>
 int rules_split(int64_t rows, int64_t span, int entries) {
   if (span <= 16384) return 1;
@@ -530,7 +533,7 @@ void launch_rules(const RulesParams& p, cudaStream_t s) {
   const int split = p.bf16 ? rules_split<__nv_bfloat16>(p.rows, span, entries) : rules_split<float>(p.rows, span, entries);
   const Part part(span, split, entries);
   // Two pieces per thread; 512 threads where two CTAs per SM take all rows (256 rows of 4,001 f32
-  // tokens with all rules: 10 us, 13 with 256 threads).
+  // tokens with all rules: 8.9 us, 12.6 with 256 threads).
   const int64_t ctas = p.rows * split;
   const int most = ctas <= 2 * 148 ? 512 : 256;
   const int threads = std::min(most, std::max(64, ((part.chunk + 2 * ve - 1) / (2 * ve) + 31) / 32 * 32));

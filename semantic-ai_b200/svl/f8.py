@@ -2,7 +2,8 @@
 
 add_norm_f8 writes such rows (svl_add_norm_f8_device), F8Linear multiplies them by an e4m3 matrix
 with a scale per 128 x 128 block (svl_f8_linear_device). Both enqueue on torch's current stream of
-the tensors' device, or on `stream`, and may be captured into CUDA graphs.
+the tensors' device, or on `stream`, and may be captured into CUDA graphs. They are for inference: inputs that
+require a gradient are taken, but outputs are detached from them.
 """
 from __future__ import annotations
 
@@ -85,7 +86,8 @@ class F8Linear:
     def __call__(self, q, scales, out_dtype=torch.float32, out=None, stream=None):
         """q: float8_e4m3fn CUDA [rows, k], 16-byte aligned rows, scales: float32 [ceil(k / 128),
         rows] (both as add_norm_f8 returns them) -> [rows, n] of out_dtype, or `out` (whose dtype
-        counts then)."""
+        counts then). The call does not wait: if a bounded wait of the product on the device ran out, only
+        check() tells, and the outputs are undefined."""
         if self.handle is None:
             raise ValueError("the F8Linear is closed")
         if stream is not None:

@@ -1,5 +1,6 @@
 """The rules between logits and token on torch tensors: penalties for repeated tokens, biases,
-grammar masks and the greedy pick (svl_logits_rules_device)."""
+grammar masks and the greedy pick (svl_logits_rules_device). For inference: logits that require a gradient are
+taken, but the outputs are detached from them."""
 from __future__ import annotations
 
 import ctypes
