@@ -110,3 +110,62 @@ def test_run_frames_with_no_token_left(svl_lib):
     assert st.position(0) == 4
     st.clear_rules(1)
     assert all(t < stt.text_card for t in gm.step([1, 2], audio[0], st))
+
+
+def test_two_states_step_at_once(svl_lib):
+    """Two e4m3 states of one model on two streams, one of them ruled, against each alone."""
+    import ctypes
+
+    import torch
+
+    from svl import _lib
+    stt, gm = toy(layers=6)
+    audio = torch.from_numpy(synth.audio_tokens(stt, 30, streams=40).astype(np.int32)).cuda()
+    text = torch.randint(0, stt.text_card, (30, 40), device="cuda", dtype=torch.int32, generator=torch.Generator(device="cuda").manual_seed(3))
+
+    def run(together):
+        states = [gm.init_state(40), gm.init_state(40)]
+        states[1].set_rules(repetition=1.5, presence=1.0, first_penalised=0, bias={3: 0.5})
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        out = torch.empty(2, 30, 40, dtype=torch.int32, device="cuda")
+        logits = torch.empty(2, 30, 40, stt.text_card, device="cuda")
+        torch.cuda.synchronize()
+        order = [(s, i) for i in range(30) for s in (0, 1)] if together else [(s, i) for s in (0, 1) for i in range(30)]
+        for s, i in order:
+            _lib.check(_lib.lib().svl_stt_step_device(gm.handle, states[s].handle, 40, *(ctypes.c_void_p(t.data_ptr()) for t in (text[i], audio[i], out[s, i], logits[s, i])),
+                                                      ctypes.c_void_p(streams[s].cuda_stream)))
+            if not together:
+                streams[s].synchronize()
+        for s in states:
+            s.check()
+        return out, logits
+
+    alone, together = run(False), run(True)
+    assert torch.equal(alone[0], together[0]) and torch.equal(alone[1], together[1])
+
+
+def test_profiling_calls_take_an_e4m3_model(svl_lib):
+    """svl_profile_kernels and svl_step_kernel_count of a ruled e4m3 state; after a reset it steps as before."""
+    import ctypes
+
+    from svl import _lib
+    stt, gm = toy()
+    st = gm.init_state(20)
+    audio = synth.audio_tokens(stt, 3, streams=20)
+    want = gm.run_frames(audio, st)
+    for which in (0, 1):
+        n = ctypes.c_int64()
+        _lib.check(_lib.lib().svl_profile_kernels(gm.handle, st.handle, 20, which, 3, None, ctypes.byref(n)))
+        assert n.value > 0
+    st.check()
+    counts = []
+    for rules in (False, True):
+        if rules:
+            st.set_rules(repetition=2.0)
+        k = ctypes.c_int32()
+        _lib.check(_lib.lib().svl_step_kernel_count(gm.handle, st.handle, 20, ctypes.byref(k)))
+        counts.append(k.value)
+    assert counts[0] == counts[1] > 20  # the rules' kernel picks the token in either
+    st.clear_rules()
+    st.reset()
+    np.testing.assert_array_equal(gm.run_frames(audio, st), want)
